@@ -554,6 +554,66 @@ int crnn_preprocess(const unsigned char* src, const crnn_crop_desc* desc, int B,
 /* bytes of device workspace crnn_preprocess needs (the per-column / per-row resampling taps) */
 long crnn_preprocess_workspace(int B, int H, int W);
 
+/* ------------------------------------------------------------------ layer norm
+ * y[m][n] = (x[m][n] - mean_m) * rstd_m * w[n] + b[n] over the last axis, rstd = 1 / sqrt(var + eps), var the population
+ * variance. x, y in dtype (fp32 or bf16) with row strides ldx, ldy >= N; w, b fp32 (either may be NULL: 1, 0);
+ * mean, rstd [M] fp32 outputs for the backward (both NULL: inference). Any M >= 0, N >= 1, any alignment of the
+ * elements' own type. */
+int crnn_layernorm_fwd(int dtype, const void* x, long ldx, const float* w, const float* b, void* y, long ldy, float* mean,
+                       float* rstd, long M, int N, float eps, void* stream);
+/* dx = rstd (g - mean(g) - xhat mean(g xhat)) (+ dres), g = dy w; dw[n] (+)= sum_m dy xhat, db[n] (+)= sum_m dy
+ * (either NULL: not computed). dres (NULL: none): the gradient that reaches x past the norm (a residual branch), added
+ * before the one rounding of dx; dx may be dres. ws: crnn_layernorm_bwd_workspace bytes. The sums over rows run in a
+ * fixed order (no atomics). */
+size_t crnn_layernorm_bwd_workspace(int dtype, long M, int N);
+int crnn_layernorm_bwd(int dtype, const void* dy, long lddy, const void* x, long ldx, const float* w, const float* mean,
+                       const float* rstd, const void* dres, long ldr, void* dx, long lddx, float* dw, float* db,
+                       int accumulate, float* ws, size_t ws_bytes, long M, int N, void* stream);
+
+/* ------------------------------------------------------------------ linear layer with its epilogue
+ * y[M][N] = act(x[M][K] . w[N][K]^T + bias[N]) + res[M][N], act one of CRNN_ACT_*; accumulation, bias, activation and
+ * residual in fp32, one rounding. x, w, y, res in dtype; bias fp32 (bias_f32 = 1) or dtype; bias, res may be NULL.
+ * z (NULL: not stored) = the pre-activation in dtype, which the backward of gelu / silu / relu reads.
+ * Any M >= 0, N, K >= 1 and element-aligned row strides: operands whose rows are not 16-byte aligned multiples of 8
+ * are first copied into ws (crnn_linear_fwd_workspace bytes, 0 for aligned ones). w stays under 2 GiB. */
+#define CRNN_ACT_NONE 0
+#define CRNN_ACT_RELU 1
+#define CRNN_ACT_GELU 2 /* z Phi(z), the erf form */
+#define CRNN_ACT_SILU 3 /* z sigmoid(z) */
+size_t crnn_linear_fwd_workspace(int dtype, const void* x, long ldx, const void* w, long ldw, long M, int N, int K);
+int crnn_linear_fwd(int dtype, const void* x, long ldx, const void* w, long ldw, const void* bias, int bias_f32, int act,
+                    const void* res, long ldr, void* y, long ldy, void* z, long ldz, void* ws, size_t ws_bytes, long M,
+                    int N, int K, void* stream);
+/* dz = dy act'(z) (z NULL: act none), dx = dz w, dw (+)= dz^T x, db (+)= sum_m dz; dx, dw, db may each be NULL. dx in
+ * dtype; dw fp32 (dw_f32 = 1) or dtype, contiguous [N][K]; db fp32 (db_f32 = 1) or dtype. accumulate needs fp32 dw, db.
+ * The sums over rows run in a fixed order. ws: crnn_linear_bwd_workspace bytes. */
+size_t crnn_linear_bwd_workspace(int dtype, const void* dy, long lddy, const void* x, long ldx, const void* w, long ldw,
+                                 int act, int need_dx, int need_dw, int need_db, long M, int N, int K);
+int crnn_linear_bwd(int dtype, const void* dy, long lddy, const void* x, long ldx, const void* w, long ldw, const void* z,
+                    long ldz, int act, void* dx, long lddx, void* dw, int dw_f32, void* db, int db_f32, int accumulate,
+                    void* ws, size_t ws_bytes, long M, int N, int K, void* stream);
+
+/* ------------------------------------------------------------------ gated linear recurrence
+ * h_t = a_t h_{t-1} + (1 - a_t) v_t, a_t = sigmoid(f_t), per channel along the sequence; y_t = h_t. f, v, y [B][T][D] in
+ * dtype, channels contiguous, batch / step strides in elements. dir 0: t = 0 .. len-1; 1: t = len-1 .. 0; 2: channels
+ * [0, D/2) forward and [D/2, D) backward in time (D even; the bidirectional encoder's [forward | reverse] rows).
+ * lengths (NULL: all T) int32 [B], clamped to [0, T]: steps t >= lengths[b] are not read and get y = 0.
+ * h0 (NULL: 0) fp32 [B][D]: the state before the first step; hT (NULL: not stored) fp32 [B][D]: the one after the last
+ * (h0 where the length is 0; hT may be h0 where the
+ * workspace is 0, e.g. for T <= 8). ckpt (NULL: inference): crnn_gated_scan_ckpt_bytes, fp32 states that the
+ * backward recomputes h from. ws: crnn_gated_scan_workspace bytes (the segment summaries of long, few sequences). */
+size_t crnn_gated_scan_ckpt_bytes(int dtype, int B, int T, int D, int dir);
+size_t crnn_gated_scan_workspace(int dtype, int B, int T, int D, int dir);
+int crnn_gated_scan_fwd(int dtype, const void* f, long fsb, long fst, const void* v, long vsb, long vst, const float* h0,
+                        const int* lengths, void* y, long ysb, long yst, float* hT, float* ckpt, float* ws,
+                        size_t ws_bytes, int B, int T, int D, int dir, void* stream);
+/* G_t = dy_t + a_{t+1} G_{t+1} (+ dhT at the last step); df_t = G_t (h_{t-1} - v_t) a_t (1 - a_t), dv_t = G_t (1 - a_t),
+ * dh0 = a_first G_first; zero at t >= lengths[b]. dhT (NULL: 0), dh0 (NULL: not stored) fp32 [B][D]. */
+int crnn_gated_scan_bwd(int dtype, const void* dy, long dsb, long dst, const void* f, long fsb, long fst, const void* v,
+                        long vsb, long vst, const int* lengths, const float* dhT, const float* ckpt, void* df, long gsb,
+                        long gst, void* dv, long wsb, long wst, float* dh0, float* ws, size_t ws_bytes, int B, int T,
+                        int D, int dir, void* stream);
+
 /* ------------------------------------------------------------------ CTC */
 /* Per-sample log-space CTC over logits [B][T][ldc] (fp32, C classes, blank = 0, input length T).
  * loss[b] = -log p(target_b); dlogits (may be NULL) = grad of the 'mean' reduction

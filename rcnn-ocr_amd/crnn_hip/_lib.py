@@ -155,6 +155,20 @@ _SIGS = {
     "crnn_preprocess": ([vp, vp, i32, i32, i32, i32, i32, vp, vp, i64, vp], i32),
     "crnn_preprocess_workspace": ([i32, i32, i32], i64),
     "crnn_attn_xent": ([vp, i32, vp, i32, i32, i32, vp, vp, i32, vp, vp], i32),
+    "crnn_layernorm_fwd": ([i32, vp, i64, vp, vp, vp, i64, vp, vp, i64, i32, f32, vp], i32),
+    "crnn_layernorm_bwd_workspace": ([i32, i64, i32], sz),
+    "crnn_layernorm_bwd": ([i32, vp, i64, vp, i64, vp, vp, vp, vp, i64, vp, i64, vp, vp, i32, vp, sz, i64, i32, vp], i32),
+    "crnn_linear_fwd_workspace": ([i32, vp, i64, vp, i64, i64, i32, i32], sz),
+    "crnn_linear_fwd": ([i32, vp, i64, vp, i64, vp, i32, i32, vp, i64, vp, i64, vp, i64, vp, sz, i64, i32, i32, vp], i32),
+    "crnn_linear_bwd_workspace": ([i32, vp, i64, vp, i64, vp, i64, i32, i32, i32, i32, i64, i32, i32], sz),
+    "crnn_linear_bwd": ([i32, vp, i64, vp, i64, vp, i64, vp, i64, i32, vp, i64, vp, i32, vp, i32, i32, vp, sz, i64, i32,
+                         i32, vp], i32),
+    "crnn_gated_scan_ckpt_bytes": ([i32, i32, i32, i32, i32], sz),
+    "crnn_gated_scan_workspace": ([i32, i32, i32, i32, i32], sz),
+    "crnn_gated_scan_fwd": ([i32, vp, i64, i64, vp, i64, i64, vp, vp, vp, i64, i64, vp, vp, vp, sz, i32, i32, i32, i32,
+                             vp], i32),
+    "crnn_gated_scan_bwd": ([i32, vp, i64, i64, vp, i64, i64, vp, i64, i64, vp, vp, vp, vp, i64, i64, vp, i64, i64, vp,
+                             vp, sz, i32, i32, i32, i32, vp], i32),
     "crnn_ctc_loss": ([vp, i32, i32, i32, i32, vp, i32, vp, vp, vp, i32, vp], i32),
     "crnn_ctc_reduce_mean": ([vp, vp, i32, vp, vp], i32),
     "crnn_ctc_greedy": ([vp, i32, i32, i32, i32, vp, vp, vp], i32),
@@ -248,6 +262,41 @@ def dtype_code(dt: torch.dtype) -> int:
     if dt == torch.float32:
         return F32
     raise ValueError(f"unsupported compute dtype {dt}")
+
+
+def call_on(t: torch.Tensor, name: str, *args):
+    """call(name, *args, stream) with t's device current and that device's current torch stream"""
+    idx = t.device.index
+    if idx == torch.cuda.current_device():
+        call(name, *args, torch.cuda.current_stream(idx).cuda_stream)
+    else:
+        with torch.cuda.device(idx):
+            call(name, *args, torch.cuda.current_stream(idx).cuda_stream)
+
+
+def rows(t: torch.Tensor):
+    """t [..., N] as M rows of N contiguous elements -> (tensor, M, row stride): t itself where its strides allow, else a
+    contiguous copy"""
+    n = t.shape[-1]
+    m = t.numel() // n if n else 0
+    if t.dim() == 2 and (t.stride(1) == 1 or n == 1) and t.stride(0) >= n:
+        return t, m, t.stride(0)
+    if not t.is_contiguous():
+        t = t.contiguous()
+    return t, m, n
+
+
+def check_operand(op: str, name: str, t, shape, dtype, device):
+    """ValueError unless t is a tensor of this shape (None: any), dtype (one or several) and device"""
+    if not isinstance(t, torch.Tensor):
+        raise ValueError(f"{op}: {name} must be a tensor, got {type(t).__name__}")
+    if shape is not None and tuple(t.shape) != tuple(shape):
+        raise ValueError(f"{op}: {name} must have shape {tuple(shape)}, got {tuple(t.shape)}")
+    ok = dtype if isinstance(dtype, tuple) else (dtype,)
+    if t.dtype not in ok:
+        raise ValueError(f"{op}: {name} must be {' or '.join(str(d) for d in ok)}, got {t.dtype}")
+    if t.device != device:
+        raise ValueError(f"{op}: {name} must be on {device}, got {t.device}")
 
 
 def require_device(t: torch.Tensor):
