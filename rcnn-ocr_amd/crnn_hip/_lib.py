@@ -264,26 +264,30 @@ def dtype_code(dt: torch.dtype) -> int:
     raise ValueError(f"unsupported compute dtype {dt}")
 
 
+_raw_stream = torch._C._cuda_getCurrentRawStream   # current_stream(i).cuda_stream without the Python Stream object (1 us)
+
+
 def call_on(t: torch.Tensor, name: str, *args):
     """call(name, *args, stream) with t's device current and that device's current torch stream"""
-    idx = t.device.index
-    if idx == torch.cuda.current_device():
-        call(name, *args, torch.cuda.current_stream(idx).cuda_stream)
+    idx = t.get_device()
+    if idx == torch._C._cuda_getDevice():
+        rc = getattr(_lib or lib(), name)(*args, _raw_stream(idx))
     else:
         with torch.cuda.device(idx):
-            call(name, *args, torch.cuda.current_stream(idx).cuda_stream)
+            rc = getattr(_lib or lib(), name)(*args, _raw_stream(idx))
+    if rc:
+        check(rc, name)
 
 
 def rows(t: torch.Tensor):
     """t [..., N] as M rows of N contiguous elements -> (tensor, M, row stride): t itself where its strides allow, else a
     contiguous copy"""
     n = t.shape[-1]
-    m = t.numel() // n if n else 0
+    if t.is_contiguous():
+        return t, t.numel() // n if n else 0, n
     if t.dim() == 2 and (t.stride(1) == 1 or n == 1) and t.stride(0) >= n:
-        return t, m, t.stride(0)
-    if not t.is_contiguous():
-        t = t.contiguous()
-    return t, m, n
+        return t, t.shape[0], t.stride(0)
+    return t.contiguous(), t.numel() // n if n else 0, n
 
 
 def check_operand(op: str, name: str, t, shape, dtype, device):
@@ -297,6 +301,15 @@ def check_operand(op: str, name: str, t, shape, dtype, device):
         raise ValueError(f"{op}: {name} must be {' or '.join(str(d) for d in ok)}, got {t.dtype}")
     if t.device != device:
         raise ValueError(f"{op}: {name} must be on {device}, got {t.device}")
+
+
+def differentiable_once(backward):
+    """torch's once_differentiable, at its price (4 us a call) only where create_graph asks for a second derivative"""
+    guarded = torch.autograd.function.once_differentiable(backward)
+
+    def run(ctx, *grads):
+        return guarded(ctx, *grads) if torch.is_grad_enabled() else backward(ctx, *grads)
+    return run
 
 
 def require_device(t: torch.Tensor):

@@ -16,57 +16,55 @@ def _bytes(n: int, device):
     return torch.empty(n, dtype=torch.uint8, device=device) if n else None
 
 
-def linear_fwd(x, weight, bias, act: int, residual, keep_z: bool):
-    """-> (y, z) of checked arguments; z (the pre-activation, x's dtype) only if keep_z and there is an activation"""
-    n, k = weight.shape
-    dt = L.dtype_code(x.dtype)
-    x2, m, ldx = L.rows(x)
-    w2, _, ldw = L.rows(weight)
-    y = torch.empty(x.shape[:-1] + (n,), dtype=x.dtype, device=x.device)
-    z = torch.empty(m, n, dtype=x.dtype, device=x.device) if keep_z and act else None
+def _forward(x2, m: int, ldx: int, shape, w2, ldw: int, bias, act: int, residual, z):
+    n, k = w2.shape
+    dt = L.dtype_code(x2.dtype)
+    y = torch.empty(shape[:-1] + (n,), dtype=x2.dtype, device=x2.device)
     r2, ldr = None, n
     if residual is not None:
         r2, _, ldr = L.rows(residual)
-    need = L.lib().crnn_linear_fwd_workspace(dt, ptr(x2), ldx, ptr(w2), ldw, m, n, k)
-    ws = _bytes(need, x.device)
-    call_on(x, "crnn_linear_fwd", dt, ptr(x2), ldx, ptr(w2), ldw, ptr(bias),
-            1 if bias is not None and bias.dtype == torch.float32 else 0, act, ptr(r2), ldr, ptr(y), n, ptr(z), n, ptr(ws), need,
+    need = L.lib().crnn_linear_fwd_workspace(dt, x2.data_ptr(), ldx, w2.data_ptr(), ldw, m, n, k)
+    ws = _bytes(need, x2.device)
+    call_on(x2, "crnn_linear_fwd", dt, x2.data_ptr(), ldx, w2.data_ptr(), ldw, ptr(bias),
+            1 if bias is not None and bias.dtype == torch.float32 else 0, act, ptr(r2), ldr, y.data_ptr(), n, ptr(z), n, ptr(ws), need,
             m, n, k)
-    return y, z
+    return y
 
 
 class _LinearFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, act, residual):
-        y, z = linear_fwd(x, weight, bias, act, residual, True)
-        ctx.save_for_backward(x, weight, z)
-        ctx.act = act
-        ctx.bias_dtype = None if bias is None else bias.dtype
+        x2, m, ldx = L.rows(x)
+        w2, _, ldw = L.rows(weight)
+        z = torch.empty(m, w2.shape[0], dtype=x.dtype, device=x.device) if act else None   # the pre-activation
+        y = _forward(x2, m, ldx, x.shape, w2, ldw, bias, act, residual, z)
+        ctx.save_for_backward(x2, w2, z)
+        ctx.geom = (x.shape, m, ldx, ldw, act, None if bias is None else bias.dtype)
         return y
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
+    @L.differentiable_once
     def backward(ctx, dy):
-        x, weight, z = ctx.saved_tensors
+        x2, w2, z = ctx.saved_tensors
         need_x, need_w, need_b, _, need_r = ctx.needs_input_grad
+        shape, m, ldx, ldw, act, bias_dtype = ctx.geom
         dx = dw = db = None
         if need_x or need_w or need_b:
-            n, k = weight.shape
-            dt = L.dtype_code(x.dtype)
-            x2, m, ldx = L.rows(x)
-            w2, _, ldw = L.rows(weight)
+            n, k = w2.shape
+            dt = L.dtype_code(x2.dtype)
+            dev = x2.device
             dy2, _, ldd = L.rows(dy)
             if need_x:
-                dx = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+                dx = torch.empty(shape, dtype=x2.dtype, device=dev)
             if need_w:
-                dw = torch.empty(n, k, dtype=weight.dtype, device=x.device)
+                dw = torch.empty(n, k, dtype=w2.dtype, device=dev)
             if need_b:
-                db = torch.empty(n, dtype=ctx.bias_dtype, device=x.device)
-            need = L.lib().crnn_linear_bwd_workspace(dt, ptr(dy2), ldd, ptr(x2), ldx, ptr(w2), ldw, ctx.act, int(need_x),
-                                                     int(need_w), int(need_b), m, n, k)
-            ws = _bytes(need, x.device)
-            call_on(x, "crnn_linear_bwd", dt, ptr(dy2), ldd, ptr(x2), ldx, ptr(w2), ldw, ptr(z), n, ctx.act, ptr(dx), k, ptr(dw),
-                    int(weight.dtype == torch.float32), ptr(db), int(ctx.bias_dtype == torch.float32), 0, ptr(ws), need, m, n, k)
+                db = torch.empty(n, dtype=bias_dtype, device=dev)
+            need = L.lib().crnn_linear_bwd_workspace(dt, dy2.data_ptr(), ldd, x2.data_ptr(), ldx, w2.data_ptr(), ldw, act, need_x,
+                                                     need_w, need_b, m, n, k)
+            ws = _bytes(need, dev)
+            call_on(x2, "crnn_linear_bwd", dt, dy2.data_ptr(), ldd, x2.data_ptr(), ldx, w2.data_ptr(), ldw, ptr(z), n, act, ptr(dx), k,
+                    ptr(dw), w2.dtype == torch.float32, ptr(db), bias_dtype == torch.float32, 0, ptr(ws), need, m, n, k)
         return dx, dw, db, None, dy if need_r else None
 
 
@@ -97,4 +95,6 @@ def linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] =
     L.require_device(x)
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, bias, residual)):
         return _LinearFn.apply(x, weight, bias, act, residual)
-    return linear_fwd(x, weight, bias, act, residual, False)[0]
+    x2, m, ldx = L.rows(x)
+    w2, _, ldw = L.rows(weight)
+    return _forward(x2, m, ldx, x.shape, w2, ldw, bias, act, residual, None)

@@ -9,45 +9,41 @@ from . import _lib as L
 from ._lib import call_on, ptr
 
 
-def layer_norm_fwd(x: torch.Tensor, weight, bias, eps: float, stats: bool):
-    """-> (y, mean, rstd) of checked arguments; mean, rstd fp32 [rows] (None unless stats)"""
-    x2, m, ldx = L.rows(x)
-    n = x.shape[-1]
-    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    mean = rstd = None
-    if stats:
-        mean, rstd = torch.empty(2, m, dtype=torch.float32, device=x.device)
-    call_on(x, "crnn_layernorm_fwd", L.dtype_code(x.dtype), ptr(x2), ldx, ptr(weight), ptr(bias), ptr(y), n, ptr(mean),
-            ptr(rstd), m, n, eps)
-    return y, mean, rstd
+def _forward(x2, m: int, ldx: int, shape, weight, bias, eps: float, stats):
+    y = torch.empty(shape, dtype=x2.dtype, device=x2.device)
+    n = shape[-1]
+    sp = ptr(stats)
+    call_on(x2, "crnn_layernorm_fwd", L.dtype_code(x2.dtype), x2.data_ptr(), ldx, ptr(weight), ptr(bias), y.data_ptr(), n, sp,
+            sp + 4 * m if stats is not None else None, m, n, eps)
+    return y
 
 
 class _LayerNormFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, eps):
-        y, mean, rstd = layer_norm_fwd(x, weight, bias, eps, True)
-        ctx.save_for_backward(x, weight, mean, rstd)
-        ctx.has_bias = bias is not None
+        x2, m, ldx = L.rows(x)
+        n = x.shape[-1]
+        stats = torch.empty(2 * m, dtype=torch.float32, device=x.device)   # mean, then rstd of every row
+        y = _forward(x2, m, ldx, x.shape, weight, bias, eps, stats)
+        ctx.save_for_backward(x2, weight, stats)
+        ctx.geom = (x.shape, m, n, ldx, L.lib().crnn_layernorm_bwd_workspace(L.dtype_code(x.dtype), m, n))
         return y
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
+    @L.differentiable_once
     def backward(ctx, dy):
-        x, weight, mean, rstd = ctx.saved_tensors
+        x2, weight, stats = ctx.saved_tensors
         need_x, need_w, need_b, _ = ctx.needs_input_grad
-        n = x.shape[-1]
-        x2, m, ldx = L.rows(x)
-        dy2, _, ldd = L.rows(dy)
-        dt = L.dtype_code(x.dtype)
-        dx = torch.empty(x.shape, dtype=x.dtype, device=x.device) if need_x else None
-        dw = torch.empty(n, dtype=torch.float32, device=x.device) if need_w else None
-        db = torch.empty(n, dtype=torch.float32, device=x.device) if need_b else None
-        ws, need = None, 0
-        if need_w or need_b:
-            need = L.lib().crnn_layernorm_bwd_workspace(dt, m, n)
-            ws = torch.empty(need // 4, dtype=torch.float32, device=x.device)
-        call_on(x, "crnn_layernorm_bwd", dt, ptr(dy2), ldd, ptr(x2), ldx, ptr(weight), ptr(mean), ptr(rstd), None, 0, ptr(dx), n,
-                ptr(dw), ptr(db), 0, ptr(ws), need, m, n)
+        shape, m, n, ldx, need = ctx.geom
+        dy, _, ldd = L.rows(dy)
+        dev = x2.device
+        dx = torch.empty(shape, dtype=x2.dtype, device=dev) if need_x else None
+        dw = torch.empty(n, dtype=torch.float32, device=dev) if need_w else None
+        db = torch.empty(n, dtype=torch.float32, device=dev) if need_b else None
+        ws = torch.empty(need // 4, dtype=torch.float32, device=dev) if need_w or need_b else None
+        sp = stats.data_ptr()
+        call_on(x2, "crnn_layernorm_bwd", L.dtype_code(x2.dtype), dy.data_ptr(), ldd, x2.data_ptr(), ldx, ptr(weight), sp, sp + 4 * m,
+                None, 0, ptr(dx), n, ptr(dw), ptr(db), 0, ptr(ws), need, m, n)
         return dx, dw, db, None
 
 
@@ -73,4 +69,5 @@ def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Opt
     if torch.is_grad_enabled() and (x.requires_grad or (weight is not None and weight.requires_grad)
                                     or (bias is not None and bias.requires_grad)):
         return _LayerNormFn.apply(x, weight, bias, float(eps))
-    return layer_norm_fwd(x, weight, bias, float(eps), False)[0]
+    x2, m, ldx = L.rows(x)
+    return _forward(x2, m, ldx, x.shape, weight, bias, float(eps), None)

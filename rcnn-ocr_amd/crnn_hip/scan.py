@@ -22,55 +22,59 @@ def _floats(nbytes: int, device):
     return torch.empty(nbytes // 4, dtype=torch.float32, device=device) if nbytes else None
 
 
-def gated_scan_fwd(f, v, h0, lengths, direction: int, want_state: bool, keep: bool, out_state=None):
-    """-> (y, hT, ckpt) of checked [B, T, D] arguments; hT if want_state (written into out_state if given), ckpt (what the
-    backward starts from) if keep"""
+def _forward(f, v, h0, lengths, direction: int, need: int, hT, ckpt):
+    """y of checked [B, T, D] arguments, channels contiguous; hT and ckpt (each may be None) are written"""
     B, T, D = f.shape
-    dt = L.dtype_code(f.dtype)
-    lib = L.lib()
     y = torch.empty(B, T, D, dtype=f.dtype, device=f.device)
-    hT = None
-    if want_state:
-        hT = out_state if out_state is not None else torch.empty(B, D, dtype=torch.float32, device=f.device)
-    ckpt = _floats(lib.crnn_gated_scan_ckpt_bytes(dt, B, T, D, direction), f.device) if keep else None
-    need = lib.crnn_gated_scan_workspace(dt, B, T, D, direction)
     ws = _floats(need, f.device)
-    f, v = _chan(f), _chan(v)
-    call_on(f, "crnn_gated_scan_fwd", dt, ptr(f), f.stride(0), f.stride(1), ptr(v), v.stride(0), v.stride(1), ptr(h0), ptr(lengths),
-            ptr(y), T * D, D, ptr(hT), ptr(ckpt), ptr(ws), need, B, T, D, direction)
-    return y, hT, ckpt
+    fs, vs = f.stride(), v.stride()
+    call_on(f, "crnn_gated_scan_fwd", L.dtype_code(f.dtype), f.data_ptr(), fs[0], fs[1], v.data_ptr(), vs[0], vs[1], ptr(h0), ptr(lengths),
+            y.data_ptr(), T * D, D, ptr(hT), ptr(ckpt), ptr(ws), need, B, T, D, direction)
+    return y
 
 
 class _GatedScanFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, f, v, h0, lengths, direction, want_state):
-        y, hT, ckpt = gated_scan_fwd(f, v, h0, lengths, direction, want_state, True)
+        B, T, D = f.shape
+        dt = L.dtype_code(f.dtype)
+        lib = L.lib()
+        f, v = _chan(f), _chan(v)
+        need = lib.crnn_gated_scan_workspace(dt, B, T, D, direction)
+        ckpt = _floats(lib.crnn_gated_scan_ckpt_bytes(dt, B, T, D, direction), f.device)   # what the backward starts from
+        hT = torch.empty(B, D, dtype=torch.float32, device=f.device) if want_state else None
+        y = _forward(f, v, h0, lengths, direction, need, hT, ckpt)
         ctx.save_for_backward(f, v, lengths, ckpt)
-        ctx.direction = direction
+        ctx.geom = (direction, need)
         ctx.set_materialize_grads(False)
         return (y, hT) if want_state else y
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
+    @L.differentiable_once
     def backward(ctx, dy, dhT=None):
         f, v, lengths, ckpt = ctx.saved_tensors
         need_f, need_v, need_h, _, _, _ = ctx.needs_input_grad
+        direction, need = ctx.geom
         B, T, D = f.shape
-        dt = L.dtype_code(f.dtype)
-        if dy is None:   # only the final state was used
-            dy = torch.zeros(B, T, D, dtype=f.dtype, device=f.device)
-        dy, f2, v2 = _chan(dy), _chan(f), _chan(v)
+        dev = f.device
+        # only the final state was used: no upstream gradient for y
+        dy = torch.zeros(B, T, D, dtype=f.dtype, device=dev) if dy is None else _chan(dy)
         if dhT is not None:
             dhT = dhT.contiguous()
-        df = torch.empty(B, T, D, dtype=f.dtype, device=f.device)
-        dv = torch.empty(B, T, D, dtype=f.dtype, device=f.device)
-        dh0 = torch.empty(B, D, dtype=torch.float32, device=f.device) if need_h else None
-        need = L.lib().crnn_gated_scan_workspace(dt, B, T, D, ctx.direction)
-        ws = _floats(need, f.device)
-        call_on(f, "crnn_gated_scan_bwd", dt, ptr(dy), dy.stride(0), dy.stride(1), ptr(f2), f2.stride(0), f2.stride(1), ptr(v2),
-                v2.stride(0), v2.stride(1), ptr(lengths), ptr(dhT), ptr(ckpt), ptr(df), T * D, D, ptr(dv), T * D, D, ptr(dh0), ptr(ws),
-                need, B, T, D, ctx.direction)
+        df = torch.empty(B, T, D, dtype=f.dtype, device=dev)
+        dv = torch.empty(B, T, D, dtype=f.dtype, device=dev)
+        dh0 = torch.empty(B, D, dtype=torch.float32, device=dev) if need_h else None
+        ws = _floats(need, dev)
+        fs, vs, ds = f.stride(), v.stride(), dy.stride()
+        call_on(f, "crnn_gated_scan_bwd", L.dtype_code(f.dtype), dy.data_ptr(), ds[0], ds[1], f.data_ptr(), fs[0], fs[1], v.data_ptr(), vs[0],
+                vs[1], ptr(lengths), ptr(dhT), ptr(ckpt), df.data_ptr(), T * D, D, dv.data_ptr(), T * D, D, ptr(dh0), ptr(ws), need, B, T, D,
+                direction)
         return df if need_f else None, dv if need_v else None, dh0, None, None, None
+
+
+def _infer(f, v, h0, lengths, direction: int, hT):
+    f, v = _chan(f), _chan(v)
+    return _forward(f, v, h0, lengths, direction, L.lib().crnn_gated_scan_workspace(L.dtype_code(f.dtype), *f.shape, direction), hT, None)
 
 
 def gated_scan(f: torch.Tensor, v: torch.Tensor, h0: Optional[torch.Tensor] = None, lengths: Optional[torch.Tensor] = None,
@@ -107,7 +111,8 @@ def gated_scan(f: torch.Tensor, v: torch.Tensor, h0: Optional[torch.Tensor] = No
         lengths = lengths.to(device=f.device, dtype=torch.int32).contiguous()
     if torch.is_grad_enabled() and (f.requires_grad or v.requires_grad or (h0 is not None and h0.requires_grad)):
         return _GatedScanFn.apply(f, v, h0, lengths, dr, return_state)
-    y, hT, _ = gated_scan_fwd(f, v, h0, lengths, dr, return_state, False)
+    hT = torch.empty(B, D, dtype=torch.float32, device=f.device) if return_state else None
+    y = _infer(f, v, h0, lengths, dr, hT)
     return (y, hT) if return_state else y
 
 
@@ -131,5 +136,7 @@ def gated_scan_step(f: torch.Tensor, v: torch.Tensor, state: torch.Tensor, out_s
         if not same and a < b + span and b < a + n:
             raise ValueError("gated_scan_step: out_state overlaps state without being it")
     L.require_device(f)
-    y, hT, _ = gated_scan_fwd(f.unsqueeze(1), v.unsqueeze(1), state.contiguous(), None, 0, True, False, out_state)
-    return y.squeeze(1), hT
+    if out_state is None:
+        out_state = torch.empty(f.shape, dtype=torch.float32, device=f.device)
+    y = _infer(f.unsqueeze(1), v.unsqueeze(1), state.contiguous(), None, 0, out_state)
+    return y.squeeze(1), out_state

@@ -97,6 +97,12 @@ template <class E> struct prefers_4w<E, std::void_t<decltype(E::kPrefer4W)>> : s
 template <class E, class = void> struct has_row8 : std::false_type {};
 template <class E> struct has_row8<E, std::void_t<decltype(E::kRow8)>> : std::bool_constant<E::kRow8> {};
 
+// optional whole-block epilogue: an EPI with `static constexpr bool kOwnTile = true` gets the wave's WM x WN accumulators at once,
+// epi.own_tile<MI, NI, WM, WN>(acc, its LDS region, lane, first row, first column), instead of one store() per fragment: it can
+// issue the loads its epilogue needs together, before the first store
+template <class E, class = void> struct has_own_tile : std::false_type {};
+template <class E> struct has_own_tile<E, std::void_t<decltype(E::kOwnTile)>> : std::bool_constant<E::kOwnTile> {};
+
 // per-wave, per-column partial statistics (sum, sum of squared deviations from the partial
 // mean) over this wave's WM accumulator rows — the BN two-pass-in-registers epilogue
 template <int MI, int NI, class EPI>
@@ -470,7 +476,9 @@ __device__ __forceinline__ void gemm256_item(LA la, LB lb, EPI epi, int M, int K
   GEMM_STAMP(2);
 
   const int mr = lane & 15, nq = 4 * (lane >> 4);
-  if constexpr (has_row8<EPI>::value && crnn_row8_on) {
+  if constexpr (has_own_tile<EPI>::value) {
+    epi.template own_tile<MI, NI, WM, WN>(acc, reinterpret_cast<float*>(smem) + wid * (64 * WN), lane, m0 + wr * WM, n0 + wc * WN);
+  } else if constexpr (has_row8<EPI>::value && crnn_row8_on) {
     row8_epilogue<MI, NI, WM, WN>(acc, epi, smem, wid, lane, m0 + wr * WM, n0 + wc * WN, kz);
   } else {
 #pragma unroll

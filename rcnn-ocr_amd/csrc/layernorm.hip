@@ -55,6 +55,26 @@ template <typename T> __device__ __forceinline__ void ldrow8(const T* row, int c
     for (int i = 0; i < 8; ++i) f[i] = c + i < n ? tof(row[c + i]) : fill;
   }
 }
+// the same, still packed (a row in flight)
+template <typename T> __device__ __forceinline__ typename VT<T>::v8 ldraw8(const T* row, int c, int n, float fill) {
+  typename VT<T>::v8 v;
+  if (c + 8 <= n) {
+    if constexpr (sizeof(T) == 2) {
+      v = *reinterpret_cast<const bf16x8_u*>(row + c);
+    } else {
+      const f32x4 a = *reinterpret_cast<const f32x4_u*>(row + c), b = *reinterpret_cast<const f32x4_u*>(row + c + 4);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        v[i] = a[i];
+        v[4 + i] = b[i];
+      }
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = c + i < n ? row[c + i] : fromf<T>(fill);
+  }
+  return v;
+}
 template <typename T> __device__ __forceinline__ void strow8(T* row, int c, int n, const float* f) {
   if (c + 8 <= n) {
     stu8<T>(row + c, f);
@@ -166,7 +186,7 @@ __global__ __launch_bounds__(ln_threads<WPR>()) void ln_fwd_kernel(const T* __re
 }
 
 template <typename T, int WPR, int KC>
-__global__ __launch_bounds__(ln_threads<WPR>()) void ln_bwd_kernel(const T* __restrict__ dy, long lddy, const T* __restrict__ x,
+__global__ __launch_bounds__(ln_threads<WPR>(), WPR == 1 ? 3 : 1) void ln_bwd_kernel(const T* __restrict__ dy, long lddy, const T* __restrict__ x,
                                                                    long ldx, const float* __restrict__ w,
                                                                    const float* __restrict__ mean, const float* __restrict__ rstd,
                                                                    const T* dres, long ldr, T* dx, long lddx,
@@ -191,20 +211,35 @@ __global__ __launch_bounds__(ln_threads<WPR>()) void ln_bwd_kernel(const T* __re
     if (w) ldrow8<float>(w, c[k], N, wv[k], 0.f);
   }
   int set = 0;
-  for (long m = (long)blockIdx.x * ln_rpb<WPR>() + (WPR == 1 ? wid : 0); m < M; m += (long)gridDim.x * ln_rpb<WPR>()) {
+  const long step = (long)gridDim.x * ln_rpb<WPR>();
+  long m = (long)blockIdx.x * ln_rpb<WPR>() + (WPR == 1 ? wid : 0);
+  typename VT<T>::v8 xr[KC], gr[KC];   // the next row, on its way while this one is worked on
+  if (m < M)
+#pragma unroll
+    for (int k = 0; k < KC; ++k) {
+      xr[k] = ldraw8<T>(x + m * ldx, c[k], N, 0.f);
+      gr[k] = ldraw8<T>(dy + m * lddy, c[k], N, 0.f);
+    }
+  for (; m < M; m += step) {
     const float mu = mean[m], rs = rstd[m];
     float xh[KC][8], g[KC][8];
 #pragma unroll
     for (int k = 0; k < KC; ++k) {
-      ldrow8<T>(x + m * ldx, c[k], N, xh[k], mu);   // mu past the end: xhat 0
-      ldrow8<T>(dy + m * lddy, c[k], N, g[k], 0.f);
+      unpack8<T>(xr[k], xh[k]);
+      unpack8<T>(gr[k], g[k]);
     }
+    if (m + step < M)
+#pragma unroll
+      for (int k = 0; k < KC; ++k) {
+        xr[k] = ldraw8<T>(x + (m + step) * ldx, c[k], N, 0.f);
+        gr[k] = ldraw8<T>(dy + (m + step) * lddy, c[k], N, 0.f);
+      }
     float s1 = 0.f, s2 = 0.f;
 #pragma unroll
     for (int k = 0; k < KC; ++k)
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        xh[k][i] = (xh[k][i] - mu) * rs;
+        xh[k][i] = (xh[k][i] - mu) * rs;   // past the end g is 0, so xhat's value there enters no sum
         sb[k][i] += g[k][i];
         sw[k][i] += g[k][i] * xh[k][i];
         g[k][i] *= wv[k][i];
@@ -412,11 +447,13 @@ LnPlan ln_plan(int N) {
   return {0, 0};
 }
 
-// workgroups of the backward: two per CU keep enough rows in flight and few partial rows to add up
+// workgroups of the backward: enough rows in flight, few partial rows to add up, and two rows a wave or more so that the
+// next one's loads run under this one's sums (65536 x 768 bf16, backward: 85 us at 2 workgroups per CU, 66 at 3, 88 at 4;
+// 32768 x 1536, 4 waves a row and fewer registers: 91, 67, 62; 1999 x 1021 fp32: 14.8 at one row a wave, 13.4 at two, 15.9 at
+// four)
 int ln_bwd_grid(long M, int N) {
   const LnPlan p = ln_plan(N);
-  const long rpb = p.wpr == 1 ? 4 : 1;
-  const long want = (M + rpb - 1) / rpb, cap = 2L * crnn_cu_count();
+  const long rows = p.wpr == 1 ? 8 : 2, want = (M + rows - 1) / rows, cap = (p.wpr == 4 && p.kc == 1 ? 4L : 3L) * crnn_cu_count();
   return (int)(want < 1 ? 1 : want < cap ? want : cap);
 }
 int ln_wide_slices(long M) {

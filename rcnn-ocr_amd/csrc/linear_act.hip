@@ -73,15 +73,18 @@ template <typename T> __device__ __forceinline__ float dact(int kind, float z) {
 }
 
 // ---------------------------------------------------------------- forward epilogue
-template <typename T, int ACT, bool ROW8 = false> struct ActEpi {
+template <typename T, int ACT, bool OWN = false> struct ActEpi {
   static constexpr bool kStats = false;
-  static constexpr bool kRow8 = ROW8;   // 8 columns per lane through the wave's LDS (gemm256.hpp row8_epilogue)
+  // the deep kernels: the wave's accumulators through its LDS, so that a lane stores 8 consecutive columns (16 bytes), and
+  // the residual's loads all in flight before the first store (one after the other, between stores that may alias them,
+  // they cost a memory latency per 64 rows x 8 columns: 139 -> see the table in DESIGN)
+  static constexpr bool kOwnTile = OWN;
   T *y, *z;
   const T* res;
   const void* bias;
   long ldy, ldz, ldr;
   int M, N, bias_f32;
-  int vec;   // y, z, res rows aligned for 4-column vectors (8-column ones with ROW8)
+  int vec;   // y, z, res, bias aligned for 16-byte vectors
   __device__ __forceinline__ float b(int n) const { return bias_f32 ? ((const float*)bias)[n] : tof(((const T*)bias)[n]); }
   __device__ __forceinline__ f32x4 b4(int n) const { return bias_f32 ? ld4f<float>((const float*)bias + n) : ld4f<T>((const T*)bias + n); }
   __device__ __forceinline__ void store(int m, int n, f32x4 v, int) const {
@@ -106,39 +109,67 @@ template <typename T, int ACT, bool ROW8 = false> struct ActEpi {
         y[m * ldy + n + r] = fromf<T>(u);
       }
   }
-  __device__ __forceinline__ void store8(int m, int n, f32x4 lo, f32x4 hi, int kz) const {
-    if constexpr (sizeof(T) == 2) {
-      if (vec && n + 8 <= N) {
-        if (m >= M) return;
+  template <int MI, int NI, int WM, int WN>
+  __device__ __forceinline__ void own_tile(const f32x4 (&acc)[MI][NI], float* stg, int lane, int rbase, int cbase) const {
+    static_assert(WM == 128 && (WN == 64 || WN == 32), "256-row tiles");
+    constexpr int CH = WN / 4;            // 16-byte chunks of a row
+    constexpr int LPR = WN / 8;           // lanes per row in the read-back
+    constexpr int RPI = 64 / LPR;         // rows per read-back instruction
+    constexpr int NIT = 64 / RPI;
+    const int mr = lane & 15, g = lane >> 4;
+    const int c = (lane % LPR) * 8, n = cbase + c, rl = lane / LPR;
+    const bool full = vec && n + 8 <= N;  // this lane's 8 columns as vectors
+    float bs[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) bs[e] = bias && n + e < N ? b(n + e) : 0.f;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      bf16x8 rv[NIT];
+      if (res && full) {
+#pragma unroll
+        for (int it = 0; it < NIT; ++it) {
+          const int m = rbase + h * 64 + it * RPI + rl;
+          rv[it] = ld8<bf16>(res + (m < M ? m : M - 1) * ldr + n);
+        }
+      }
+#pragma unroll
+      for (int ii = 0; ii < MI / 2; ++ii)
+#pragma unroll
+        for (int j = 0; j < NI; ++j) {
+          const int r = ii * 16 + mr, q = (4 * j + g) ^ (r & (CH - 1));
+          *reinterpret_cast<f32x4*>(stg + r * WN + 4 * q) = acc[h * (MI / 2) + ii][j];
+        }
+#pragma unroll
+      for (int it = 0; it < NIT; ++it) {
+        const int r = it * RPI + rl, m = rbase + h * 64 + r;
+        const int q0 = (c / 4) ^ (r & (CH - 1)), q1 = (c / 4 + 1) ^ (r & (CH - 1));
+        const f32x4 lo = *reinterpret_cast<const f32x4*>(stg + r * WN + 4 * q0);
+        const f32x4 hi = *reinterpret_cast<const f32x4*>(stg + r * WN + 4 * q1);
         float u[8];
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          u[r] = lo[r];
-          u[4 + r] = hi[r];
+        for (int e = 0; e < 4; ++e) {
+          u[e] = lo[e] + bs[e];
+          u[4 + e] = hi[e] + bs[4 + e];
         }
-        if (bias) {
-          const f32x4 b0 = b4(n), b1 = b4(n + 4);
+        if (m < M && full) {
+          if (z) st8<bf16>(z + m * ldz + n, pack8<bf16>(u));
 #pragma unroll
-          for (int r = 0; r < 4; ++r) {
-            u[r] += b0[r];
-            u[4 + r] += b1[r];
+          for (int e = 0; e < 8; ++e) u[e] = act<bf16, ACT>(u[e]);
+          if (res) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) u[e] += (float)rv[it][e];
+          }
+          st8<bf16>(y + m * ldy + n, pack8<bf16>(u));
+        } else if (m < M) {
+          for (int e = 0; e < 8 && n + e < N; ++e) {
+            if (z) z[m * ldz + n + e] = (bf16)u[e];
+            float o = act<bf16, ACT>(u[e]);
+            if (res) o += (float)res[m * ldr + n + e];
+            y[m * ldy + n + e] = (bf16)o;
           }
         }
-        if (z) st8<T>(z + m * ldz + n, pack8<T>(u));
-#pragma unroll
-        for (int r = 0; r < 8; ++r) u[r] = act<T, ACT>(u[r]);
-        if (res) {
-          float q[8];
-          unpack8<T>(ld8<T>(res + m * ldr + n), q);
-#pragma unroll
-          for (int r = 0; r < 8; ++r) u[r] += q[r];
-        }
-        st8<T>(y + m * ldy + n, pack8<T>(u));
-        return;
       }
     }
-    store(m, n, lo, kz);
-    store(m, n + 4, hi, kz);
   }
   __device__ __forceinline__ void stats(int, int, f32x4, f32x4) const {}
 };
@@ -157,48 +188,85 @@ long max_rows(long ld, int es) {
   return r >= 256 ? r / 256 * 256 : r;
 }
 
-// dst[rows][cols8] (zero behind cols) = src[rows][ld]
-template <typename T>
-__global__ __launch_bounds__(256) void pad_copy_kernel(const T* __restrict__ src, long ld, T* __restrict__ dst, long rows, int cols,
-                                                       int cols8) {
-  const long n8 = rows * (cols8 / 8);
-  for (long i = blockIdx.x * 256L + threadIdx.x; i < n8; i += gridDim.x * 256L) {
-    const long r = i / (cols8 / 8);
-    const int c = (int)(i - r * (cols8 / 8)) * 8;
-    float v[8];
+// columns c .. c+7 of a row of n columns at an element-aligned address, zero past its end
+typedef bf16x8 bf16x8_u __attribute__((aligned(2)));
+typedef f32x4 f32x4_u __attribute__((aligned(4)));
+template <typename T> __device__ __forceinline__ void ldrow8(const T* row, int c, int n, float* f) {
+  if (c + 8 <= n) {
+    if constexpr (sizeof(T) == 2) {
+      const bf16x8 v = *reinterpret_cast<const bf16x8_u*>(row + c);
+      unpack8<T>(v, f);
+    } else {
+      const f32x4 a = *reinterpret_cast<const f32x4_u*>(row + c), b = *reinterpret_cast<const f32x4_u*>(row + c + 4);
 #pragma unroll
-    for (int e = 0; e < 8; ++e) v[e] = c + e < cols ? tof(src[r * ld + c + e]) : 0.f;
-    st8<T>(dst + r * cols8 + c, pack8<T>(v));
+      for (int e = 0; e < 4; ++e) {
+        f[e] = a[e];
+        f[4 + e] = b[e];
+      }
+    }
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) f[e] = c + e < n ? tof(row[c + e]) : 0.f;
   }
 }
-template <typename T> int pad_copy(const void* src, long ld, void* dst, long rows, int cols, hipStream_t st) {
-  const long n8 = rows * (round8i(cols) / 8);
-  if (n8 == 0) return 0;
-  hipLaunchKernelGGL(pad_copy_kernel<T>, dim3(grid_for(n8)), dim3(256), 0, st, (const T*)src, ld, (T*)dst, rows, cols, round8i(cols));
+
+// dst[rows][cols8] (zero behind cols) = src[rows][ld], up to two matrices in one launch (blockIdx.y)
+struct PadJob {
+  const void* src;
+  void* dst;
+  long ld, rows;
+  int cols;
+};
+template <typename T> __global__ __launch_bounds__(256) void pad_copy_kernel(PadJob j0, PadJob j1) {
+  const PadJob j = blockIdx.y ? j1 : j0;
+  const int c8 = (j.cols + 7) / 8;
+  const long n8 = j.rows * c8;
+  for (long i = blockIdx.x * 256L + threadIdx.x; i < n8; i += gridDim.x * 256L) {
+    const long r = i / c8;
+    const int c = (int)(i - r * c8) * 8;
+    float v[8];
+    ldrow8<T>((const T*)j.src + r * j.ld, c, j.cols, v);
+    st8<T>((T*)j.dst + (r * c8 + c / 8) * 8, pack8<T>(v));
+  }
+}
+// copies the given jobs (src NULL: none)
+template <typename T> int pad_copy(PadJob a, PadJob b, hipStream_t st) {
+  if (!a.src) {
+    a = b;
+    b.src = nullptr;
+  }
+  if (!a.src) return 0;
+  const long na = a.rows * (round8i(a.cols) / 8), nb = b.src ? b.rows * (round8i(b.cols) / 8) : 0;
+  hipLaunchKernelGGL(pad_copy_kernel<T>, dim3(grid_for(na > nb ? na : nb, 256, 4096), b.src ? 2 : 1), dim3(256), 0, st, a, b);
   return (int)hipGetLastError();
 }
 
 size_t up256(size_t n) { return (n + 255) & ~(size_t)255; }
 
 // ---------------------------------------------------------------- tile plans
-// bf16: the deep 256-row kernels where their tiles alone fill three quarters of the CUs, else the register-staged ones;
-// fp32 (exact-fp32 MFMA): register-staged
-template <typename T, class LA, class LB, class E, class E8>
-int tiles_run(const LA& la, const LB& lb, const E& ep, const E8& ep8, bool row8, int M, int N, int K, hipStream_t st) {
+// Products with rows as outputs (forward, dx). bf16: the deep 256-row kernels where their tiles fill three quarters of the
+// CUs; a round of 256 x 256 tiles costs 1.4 rounds of 256 x 128 ones, so the fewer weighted rounds win (32768 x 768 x 1536:
+// 86 us at 2 rounds of the former, 94 at 3 of the latter; 8192 x 1024 x 512: 24 at half a round, 20 at a whole one).
+// Else 64 x 64 register-staged tiles where there is one per CU (4096 x 512 x 512: 12.8 us; 256 x 128 tiles 19.8, 128 x 128
+// 19.8, 32 x 32 13.6), else 32 x 32 (500 x 520 x 512: 8.0 against 9.1). fp32 (exact-fp32 MFMA, 1/16 of the bf16 rate): 64 x 64
+// at four per CU or more (8192 x 1024 x 512: 84.8 us, 128 x 128 83.0, 32 x 32 101), else 32 x 32 with 64-deep stages
+// (1032 x 1024 x 512: 22.6 against 27.4 of 64 x 64; 304 x 520 x 1000: 13.1 against 28.7).
+template <typename T, int ACT, class LA, class LB>
+int tiles_run(const LA& la, const LB& lb, const ActEpi<T, ACT>& ep, int M, int N, int K, hipStream_t st) {
+  const long cu = crnn_cu_count(), t64 = (long)((M + 63) / 64) * ((N + 63) / 64);
   if constexpr (sizeof(T) == 2) {
-    const long cu = crnn_cu_count();
     const long t256 = (long)((M + 255) / 256) * ((N + 255) / 256), t128 = (long)((M + 255) / 256) * ((N + 127) / 128);
-    if (K >= 256) {
-      if (N >= 256 && t256 * 4 >= cu * 3)
-        return row8 ? launch256<256, 256>(la, lb, ep8, M, N, K, st) : launch256<256, 256>(la, lb, ep, M, N, K, st);
-      if (N >= 128 && t128 * 4 >= cu * 3)
-        return row8 ? launch256<256, 128>(la, lb, ep8, M, N, K, st) : launch256<256, 128>(la, lb, ep, M, N, K, st);
+    if (K >= 256 && N >= 128 && t128 * 4 >= cu * 3) {
+      const ActEpi<T, ACT, true> eo{ep.y, ep.z, ep.res, ep.bias, ep.ldy, ep.ldz, ep.ldr, ep.M, ep.N, ep.bias_f32, ep.vec};
+      if ((t256 + cu - 1) / cu * 7 <= (t128 + cu - 1) / cu * 5) return launch256<256, 256>(la, lb, eo, M, N, K, st);
+      return launch256<256, 128>(la, lb, eo, M, N, K, st);
     }
+    if (t64 >= cu) return launch<T, 64, 64>(la, lb, ep, M, N, K, 1, st);
+    return launch<T, 32, 32>(la, lb, ep, M, N, K, 1, st);
+  } else {
+    if (t64 >= 4 * cu) return launch<T, 64, 64>(la, lb, ep, M, N, K, 1, st);
+    return launch<T, 32, 32, 64>(la, lb, ep, M, N, K, 1, st);
   }
-  const long work = (long)M * N;
-  if (M >= 128 && N >= 128 && work >= 128L * 128 * 128) return launch<T, 128, 128>(la, lb, ep, M, N, K, 1, st);
-  if (work >= 64L * 64 * 128) return launch<T, 64, 64>(la, lb, ep, M, N, K, 1, st);
-  return launch<T, 32, 32>(la, lb, ep, M, N, K, 1, st);
 }
 
 template <typename T, int ACT>
@@ -214,8 +282,7 @@ int fwd_act(const T* x, long ldx, const T* w, long ldw, const void* bias, int bi
     const RowMajorK<T> lb{w, (int)ldw, N, K8};
     const ActEpi<T, ACT> ep{y + m0 * ldy, z ? z + m0 * ldz : nullptr, res ? res + m0 * ldr : nullptr, bias, ldy, ldz, ldr, m, N,
                             bias_f32, al};
-    const ActEpi<T, ACT, true> ep8{ep.y, ep.z, ep.res, bias, ldy, ldz, ldr, m, N, bias_f32, al};
-    const int rc = tiles_run<T>(la, lb, ep, ep8, al, m, N, K8, st);
+    const int rc = tiles_run<T, ACT>(la, lb, ep, m, N, K8, st);
     if (rc) return rc;
   }
   return 0;
@@ -226,19 +293,20 @@ int fwd_t(const void* x, long ldx, const void* w, long ldw, const void* bias, in
           void* y, long ldy, void* z, long ldz, char* ws, long M, int N, int K, hipStream_t st) {
   const int K8 = round8i(K);
   const T *xp = (const T*)x, *wp = (const T*)w;
+  PadJob jx = {}, jw = {};
   if (!direct(x, ldx, K, sizeof(T))) {
-    const int rc = pad_copy<T>(x, ldx, ws, M, K, st);
-    if (rc) return rc;
+    jx = {x, ws, ldx, M, K};
     xp = (const T*)ws;
     ldx = K8;
     ws += up256((size_t)M * K8 * sizeof(T));
   }
   if (!direct(w, ldw, K, sizeof(T))) {
-    const int rc = pad_copy<T>(w, ldw, ws, N, K, st);
-    if (rc) return rc;
+    jw = {w, ws, ldw, N, K};
     wp = (const T*)ws;
     ldw = K8;
   }
+  const int rc = pad_copy<T>(jx, jw, st);
+  if (rc) return rc;
 #define FWD(A) fwd_act<T, A>(xp, ldx, wp, ldw, bias, bias_f32, (const T*)res, ldr, (T*)y, ldy, (T*)z, ldz, M, N, K8, st)
   if (kind == CRNN_ACT_RELU) return FWD(CRNN_ACT_RELU);
   if (kind == CRNN_ACT_GELU) return FWD(CRNN_ACT_GELU);
@@ -263,14 +331,12 @@ __global__ __launch_bounds__(256) void dz_kernel(const T* __restrict__ dy, long 
   if (n < N8)
     for (long m = (long)blockIdx.y * 8 + rl; m < M; m += 8L * gridDim.y) {
       float g[8], q[8];
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        g[e] = n + e < N ? tof(dy[m * lddy + n + e]) : 0.f;
-        q[e] = z && n + e < N ? tof(z[m * ldz + n + e]) : 0.f;
-      }
-      if (z)
+      ldrow8<T>(dy + m * lddy, n, N, g);
+      if (z) {
+        ldrow8<T>(z + m * ldz, n, N, q);
 #pragma unroll
         for (int e = 0; e < 8; ++e) g[e] *= dact<T>(kind, q[e]);
+      }
 #pragma unroll
       for (int e = 0; e < 8; ++e) s[e] += g[e];
       if (dz) st8<T>(dz + m * N8 + n, pack8<T>(g));
@@ -293,32 +359,6 @@ template <typename O> __device__ __forceinline__ void put(O* o, float v, int acc
   else *o = fromf<O>(v);
 }
 
-// out[n] (+)= sum_g part[g][n]: 64 columns per workgroup, 16 row lanes, fixed order
-template <typename O>
-__global__ __launch_bounds__(1024) void db_reduce_kernel(const float* __restrict__ part, int G, int N, O* __restrict__ out, int accumulate) {
-  __shared__ float red[16][64];
-  const int col = threadIdx.x & 63, rl = threadIdx.x >> 6, n = blockIdx.x * 64 + col;
-  float s = 0.f;
-  if (n < N) {
-    int g = rl;
-    for (; g + 7 * 16 < G; g += 8 * 16) {
-      float v[8];
-#pragma unroll
-      for (int u = 0; u < 8; ++u) v[u] = part[(size_t)(g + 16 * u) * N + n];
-#pragma unroll
-      for (int u = 0; u < 8; ++u) s += v[u];
-    }
-    for (; g < G; g += 16) s += part[(size_t)g * N + n];
-  }
-  red[rl][col] = s;
-  __syncthreads();
-  if (rl == 0 && n < N) {
-#pragma unroll
-    for (int r = 1; r < 16; ++r) s += red[r][col];
-    put<O>(out + n, s, accumulate);
-  }
-}
-
 // split-K partials of dw into fp32 slabs [S][Nr][Kc] (whole vectors), then one fixed-order sum into dw [N][K]
 struct SlabEpi {
   static constexpr bool kStats = false;
@@ -329,28 +369,51 @@ struct SlabEpi {
   }
   __device__ __forceinline__ void stats(int, int, f32x4, f32x4) const {}
 };
-template <typename O>
-__global__ __launch_bounds__(256) void dw_reduce_kernel(const float* __restrict__ ws, int S, int Nr, int Kc, O* __restrict__ dw, int N,
-                                                        int K, int accumulate) {
+// the last pass of the backward, one launch: workgroups [0, wblocks) add the S slabs into dw [N][K], the others G partial rows
+// of the column sums into db (64 columns each, 4 row lanes); every sum in a fixed order
+template <typename OW, typename OB>
+__global__ __launch_bounds__(256) void reduce_kernel(const float* __restrict__ slab, int S, int Nr, int Kc, OW* __restrict__ dw,
+                                                     int wblocks, const float* __restrict__ part, int G, OB* __restrict__ db, int N,
+                                                     int K, int accumulate) {
+  if ((int)blockIdx.x >= wblocks) {
+    __shared__ float red[4][64];
+    const int col = threadIdx.x & 63, rl = threadIdx.x >> 6, n = ((int)blockIdx.x - wblocks) * 64 + col;
+    float s = 0.f;
+    if (n < N) {
+      int g = rl;
+      for (; g + 15 * 4 < G; g += 16 * 4) {
+        float v[16];
+#pragma unroll
+        for (int u = 0; u < 16; ++u) v[u] = part[(size_t)(g + 4 * u) * N + n];
+#pragma unroll
+        for (int u = 0; u < 16; ++u) s += v[u];
+      }
+      for (; g < G; g += 4) s += part[(size_t)g * N + n];
+    }
+    red[rl][col] = s;
+    __syncthreads();
+    if (rl == 0 && n < N) put<OB>(db + n, s + red[1][col] + red[2][col] + red[3][col], accumulate);
+    return;
+  }
   const long total = (long)Nr * Kc;
-  for (long i4 = blockIdx.x * 256L + threadIdx.x; 4 * i4 < total; i4 += gridDim.x * 256L) {
+  for (long i4 = blockIdx.x * 256L + threadIdx.x; 4 * i4 < total; i4 += wblocks * 256L) {
     const long i = 4 * i4;
     f32x4 s = {0.f, 0.f, 0.f, 0.f};
     int z = 0;
     for (; z + 8 <= S; z += 8) {
       f32x4 v[8];
 #pragma unroll
-      for (int q = 0; q < 8; ++q) v[q] = *reinterpret_cast<const f32x4*>(ws + (size_t)(z + q) * total + i);
+      for (int q = 0; q < 8; ++q) v[q] = *reinterpret_cast<const f32x4*>(slab + (size_t)(z + q) * total + i);
 #pragma unroll
       for (int q = 0; q < 8; ++q) s += v[q];
     }
-    for (; z < S; ++z) s += *reinterpret_cast<const f32x4*>(ws + (size_t)z * total + i);
+    for (; z < S; ++z) s += *reinterpret_cast<const f32x4*>(slab + (size_t)z * total + i);
     const int n = (int)(i / Kc), k = (int)(i - (long)n * Kc);   // Kc % 8 == 0: the four share a row
     if (n >= N) continue;
-    O* o = dw + (size_t)n * K + k;
+    OW* o = dw + (size_t)n * K + k;
 #pragma unroll
     for (int e = 0; e < 4; ++e)
-      if (k + e < K) put<O>(o + e, s[e], accumulate);
+      if (k + e < K) put<OW>(o + e, s[e], accumulate);
   }
 }
 
@@ -360,17 +423,30 @@ int dz_slices(long M, int N) {
   long g = (2L * crnn_cu_count() + cb - 1) / cb;
   const long most = (M + 31) / 32;
   if (g > most) g = most;
-  if (g > 256) g = 256;
+  if (g > 128) g = 128;
   return (int)(g < 1 ? 1 : g);
 }
-// K splits of one launch of the weight gradient over `rows` rows
-int dw_splits(int Nr, int Kc, long rows) {
-  const long tiles = (long)((Nr + 127) / 128) * ((Kc + 127) / 128);
-  long s = (crnn_cu_count() + tiles - 1) / tiles;
-  const long smax = (rows + 16 * 64 - 1) / (16 * 64);
-  if (s > smax) s = smax;
-  if (s < 1) s = 1;
-  return eff_splits((int)rows, (int)s);
+// The weight gradient over `rows` rows: tile and K splits. Its outputs are few and its sum is long, so K is split until the
+// chip is full, as long as a split keeps enough of the sum to be worth its slab (written and read once as fp32). bf16: the deep
+// 256 x 256 kernel at one workgroup per CU if a split keeps 1024 rows (768 x 1536 over 32768: 75 us in 14 splits; 128 x 128
+// 100 in 7), else 128 x 128 at two per CU if it keeps 512 (1024 x 512 over 8192: 21 in 16; 64 x 64 23, 256 x 256 23 in 32), else
+// 64 x 64 (512 x 512 over 4096: 10.9 in 8; 128 x 128 11.6). fp32: 64 x 64 at four per CU (1024 x 512 over 1032: 19.9; 128 x 128
+// 30.7).
+struct DwPlan { int tile, splits; };
+DwPlan dw_plan(int es, int Nr, int Kc, long rows) {
+  const long cu = crnn_cu_count();
+  auto tiles = [&](int b) { return (long)((Nr + b - 1) / b) * ((Kc + b - 1) / b); };
+  auto split = [&](long wg, long least) {   // splits to reach wg workgroups, each of `least` rows or more
+    const long s = wg < 1 ? 1 : wg, most = rows / least < 1 ? 1 : rows / least;
+    return eff_splits((int)rows, (int)(s < most ? s : most));
+  };
+  if (es == 2) {
+    const long s256 = cu / tiles(256), s128 = 2 * cu / tiles(128);
+    if (s256 >= 1 ? rows / s256 >= 1024 : true) return {256, split(s256, 1024)};
+    if (s128 >= 1 && rows / s128 >= 512) return {128, split(s128, 512)};
+    return {64, split(2 * cu / tiles(64), 256)};
+  }
+  return {64, split(4 * cu / tiles(64), 256)};
 }
 
 // the layout of crnn_linear_bwd's workspace
@@ -392,7 +468,7 @@ BwdPlan bwd_plan(int dtype, const void* dy, long lddy, const void* x, long ldx, 
   const long ldz_ = p.own_dz ? p.N8 : lddy, ldx_ = p.copy_x ? p.K8 : ldx;
   if (need_dw && M > 0) {
     const long step = max_rows(ldz_ > ldx_ ? ldz_ : ldx_, es);
-    for (long m0 = 0; m0 < M; m0 += step) p.slabs += dw_splits(p.N8, p.K8, M - m0 < step ? M - m0 : step);
+    for (long m0 = 0; m0 < M; m0 += step) p.slabs += dw_plan(es, p.N8, p.K8, M - m0 < step ? M - m0 : step).splits;
   }
   size_t o = 0;
   p.o_dz = o;
@@ -428,24 +504,21 @@ int bwd_t(const BwdPlan& p, const void* dy, long lddy, const void* x, long ldx, 
       ldd = p.N8;
     }
   }
-  if (db) {
-    const int G = M > 0 ? p.slices : 0;
-    const dim3 grid((N + 63) / 64);
-    if (db_f32) hipLaunchKernelGGL(db_reduce_kernel<float>, grid, dim3(1024), 0, st, part, G, N, (float*)db, accumulate);
-    else hipLaunchKernelGGL(db_reduce_kernel<T>, grid, dim3(1024), 0, st, part, G, N, (T*)db, accumulate);
-    if ((rc = (int)hipGetLastError())) return rc;
-  }
-  if (p.copy_x && M > 0) {
-    if ((rc = pad_copy<T>(x, ldx, ws + p.o_x, M, K, st))) return rc;
-    xp = (const T*)(ws + p.o_x);
-    ldx = p.K8;
-  }
-  if (dx && M > 0) {
+  if (M > 0) {
+    PadJob jx = {}, jw = {};
+    if (p.copy_x) {
+      jx = {x, ws + p.o_x, ldx, M, K};
+      xp = (const T*)(ws + p.o_x);
+      ldx = p.K8;
+    }
     if (p.copy_w) {
-      if ((rc = pad_copy<T>(w, ldw, ws + p.o_w, N, K, st))) return rc;
+      jw = {w, ws + p.o_w, ldw, N, K};
       wp = (const T*)(ws + p.o_w);
       ldw = p.K8;
     }
+    if ((rc = pad_copy<T>(jx, jw, st))) return rc;
+  }
+  if (dx && M > 0) {
     const long step = max_rows(ldd, sizeof(T));
     const bool al = aligned16(dx) && lddx * (long)sizeof(T) % 16 == 0;
     for (long m0 = 0; m0 < M; m0 += step) {
@@ -453,28 +526,45 @@ int bwd_t(const BwdPlan& p, const void* dy, long lddy, const void* x, long ldx, 
       const RowMajorK<T> la{dzp + m0 * ldd, (int)ldd, m, p.N8};
       const ColMajorK<T> lb{wp, (int)ldw, p.K8, N};
       const ActEpi<T, CRNN_ACT_NONE> ep{(T*)dx + m0 * lddx, nullptr, nullptr, nullptr, lddx, 0, 0, m, K, 0, al};
-      const ActEpi<T, CRNN_ACT_NONE, true> ep8{ep.y, nullptr, nullptr, nullptr, lddx, 0, 0, m, K, 0, al};
-      if ((rc = tiles_run<T>(la, lb, ep, ep8, al, m, K, p.N8, st))) return rc;
+      if ((rc = tiles_run<T, CRNN_ACT_NONE>(la, lb, ep, m, K, p.N8, st))) return rc;
     }
   }
-  if (dw) {
-    float* slab = (float*)(ws + p.o_slab);
-    int s0 = 0;
-    if (M > 0) {
-      const long step = max_rows(ldd > ldx ? ldd : ldx, sizeof(T));
-      for (long m0 = 0; m0 < M; m0 += step) {
-        const int m = (int)(M - m0 < step ? M - m0 : step);
-        const int S = dw_splits(p.N8, p.K8, m);
-        const ColMajorK<T> la{dzp + m0 * ldd, (int)ldd, p.N8, m};
-        const ColMajorK<T> lb{xp + m0 * ldx, (int)ldx, p.K8, m};
-        const SlabEpi ep{slab + (size_t)s0 * p.N8 * p.K8, p.N8, p.K8};
-        if ((rc = launch<T, 128, 128>(la, lb, ep, p.N8, p.K8, m, S, st))) return rc;
-        s0 += S;
+  const float* slab = (const float*)(ws + p.o_slab);
+  int S = 0;
+  if (dw && M > 0) {
+    const long step = max_rows(ldd > ldx ? ldd : ldx, sizeof(T));
+    for (long m0 = 0; m0 < M; m0 += step) {
+      const int m = (int)(M - m0 < step ? M - m0 : step);
+      const DwPlan d = dw_plan(sizeof(T), p.N8, p.K8, m);
+      const ColMajorK<T> la{dzp + m0 * ldd, (int)ldd, p.N8, m};
+      const ColMajorK<T> lb{xp + m0 * ldx, (int)ldx, p.K8, m};
+      const SlabEpi ep{(float*)(ws + p.o_slab) + (size_t)S * p.N8 * p.K8, p.N8, p.K8};
+      if constexpr (sizeof(T) == 2) {
+        if (d.tile == 256) rc = launch256<256, 256>(la, lb, ep, p.N8, p.K8, m, st, d.splits);
+        else if (d.tile == 128) rc = launch<T, 128, 128>(la, lb, ep, p.N8, p.K8, m, d.splits, st);
+        else rc = launch<T, 64, 64>(la, lb, ep, p.N8, p.K8, m, d.splits, st);
+      } else {
+        rc = launch<T, 64, 64>(la, lb, ep, p.N8, p.K8, m, d.splits, st);
       }
+      if (rc) return rc;
+      S += d.splits;
     }
-    const int blocks = grid_for((long)p.N8 * p.K8 / 4, 256, 2048);
-    if (dw_f32) hipLaunchKernelGGL(dw_reduce_kernel<float>, dim3(blocks), dim3(256), 0, st, slab, s0, p.N8, p.K8, (float*)dw, N, K, accumulate);
-    else hipLaunchKernelGGL(dw_reduce_kernel<T>, dim3(blocks), dim3(256), 0, st, slab, s0, p.N8, p.K8, (T*)dw, N, K, accumulate);
+  }
+  if (dw || db) {
+    const int wb = dw ? grid_for((long)p.N8 * p.K8 / 4, 256, 2048) : 0, bb = db ? (N + 63) / 64 : 0, G = M > 0 ? p.slices : 0;
+    auto go = [&](auto ow, auto ob) {
+      typedef decltype(ow) OW;
+      typedef decltype(ob) OB;
+      hipLaunchKernelGGL((reduce_kernel<OW, OB>), dim3(wb + bb), dim3(256), 0, st, slab, S, p.N8, p.K8, (OW*)dw, wb, part, G, (OB*)db,
+                         N, K, accumulate);
+    };
+    if (dw_f32 || sizeof(T) == 4) {
+      if (db_f32 || sizeof(T) == 4) go(float(), float());
+      else go(float(), bf16());
+    } else {
+      if (db_f32) go(bf16(), float());
+      else go(bf16(), bf16());
+    }
     rc = (int)hipGetLastError();
   }
   return rc;

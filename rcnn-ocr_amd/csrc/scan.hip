@@ -20,46 +20,37 @@
 
 namespace {
 
-constexpr int L = 8;   // steps a wave holds
+constexpr int L = 4;      // steps a wave holds
+constexpr int kWmax = 8;  // waves of the widest tile
+// channels of a lane: 4 bytes, 256 a wave and step (wider lanes leave fewer waves: 37 x 301 x 333 fp32, forward / backward 20.6 /
+// 24.7 us at one channel, 21.8 / 26.2 at two; 2 x 16384 x 1024 bf16 70 / 99 at two, 212 / 202 at four)
+template <typename T> constexpr int vec_of() { return sizeof(T) == 2 ? 2 : 1; }
 
 // VEC consecutive channels at an element-aligned address
 template <typename T, int VEC> struct Raw;
-template <> struct Raw<bf16, 1> { typedef unsigned short t; };
-template <> struct Raw<bf16, 2> { typedef unsigned short t __attribute__((ext_vector_type(2))); };
-template <> struct Raw<float, 1> { typedef float t; };
-template <> struct Raw<float, 2> { typedef float t __attribute__((ext_vector_type(2))); };
+template <int VEC> struct Raw<bf16, VEC> { typedef unsigned short t __attribute__((ext_vector_type(VEC))); };
+template <int VEC> struct Raw<float, VEC> { typedef float t __attribute__((ext_vector_type(VEC))); };
 template <typename T, int VEC> struct RawU {   // the same, element-aligned
   typedef typename Raw<T, VEC>::t t __attribute__((aligned(sizeof(T))));
 };
 
 template <typename T, int VEC> __device__ __forceinline__ float elem(const typename Raw<T, VEC>::t& r, int i) {
-  if constexpr (sizeof(T) == 2) {
-    unsigned short u;
-    if constexpr (VEC == 1) u = r;
-    else u = r[i];
-    return __uint_as_float((unsigned)u << 16);
-  } else {
-    if constexpr (VEC == 1) return r;
-    else return r[i];
-  }
+  if constexpr (sizeof(T) == 2) return __uint_as_float((unsigned)r[i] << 16);
+  else return r[i];
 }
 template <typename T, int VEC> __device__ __forceinline__ void set_elem(typename Raw<T, VEC>::t& r, int i, float v) {
-  if constexpr (sizeof(T) == 2) {
-    const unsigned short u = __builtin_bit_cast(unsigned short, (bf16)v);
-    if constexpr (VEC == 1) r = u;
-    else r[i] = u;
-  } else {
-    if constexpr (VEC == 1) r = v;
-    else r[i] = v;
-  }
+  if constexpr (sizeof(T) == 2) r[i] = __builtin_bit_cast(unsigned short, (bf16)v);
+  else r[i] = v;
 }
 // nv: this lane's channels that exist (0 .. VEC)
 template <typename T, int VEC> __device__ __forceinline__ typename Raw<T, VEC>::t ldv(const T* p, int nv) {
   typename Raw<T, VEC>::t r = {};
   if (nv == VEC) {
     r = *reinterpret_cast<const typename RawU<T, VEC>::t*>(p);
-  } else if (nv > 0) {   // VEC = 2, one channel left
-    set_elem<T, VEC>(r, 0, tof(p[0]));
+  } else {
+#pragma unroll
+    for (int i = 0; i < VEC - 1; ++i)
+      if (i < nv) set_elem<T, VEC>(r, i, tof(p[i]));
   }
   return r;
 }
@@ -69,8 +60,10 @@ template <typename T, int VEC> __device__ __forceinline__ void stv(T* p, int nv,
 #pragma unroll
     for (int i = 0; i < VEC; ++i) set_elem<T, VEC>(r, i, v[i]);
     *reinterpret_cast<typename RawU<T, VEC>::t*>(p) = r;
-  } else if (nv > 0) {
-    p[0] = fromf<T>(v[0]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < VEC - 1; ++i)
+      if (i < nv) p[i] = fromf<T>(v[i]);
   }
 }
 
@@ -129,34 +122,51 @@ template <int VEC> __device__ __forceinline__ Who who(const ScanArgs& a) {
 // position in time of walking step u
 __device__ __forceinline__ int at(const Who& w, int u) { return w.rev && u < w.len ? w.len - 1 - u : u; }
 
-// compose the summaries of segments s0, s0 + ds, .. (n of them) onto h, eight loads in flight
-template <int VEC> __device__ __forceinline__ void compose(const ScanArgs& a, const Who& w, int s0, int ds, int n, float* h) {
+// The state (or, going back, the gradient) that enters a segment: `first` through the n summaries s0, s0 + ds, .. before it.
+// The waves of the workgroup compose a share each, eight loads in flight, and join in LDS (ex): with one wave doing all of
+// them this was 4 memory latencies of every workgroup of 2 x 16384 x 1024 in 32 segments.
+template <int VEC, int W>
+__device__ __forceinline__ void entering(const ScanArgs& a, const Who& w, const float* first, int s0, int ds, int n,
+                                         float (*ex)[VEC][64], float* h) {
+  const int lane = threadIdx.x & 63, wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+#pragma unroll
+  for (int i = 0; i < VEC; ++i) h[i] = first && i < w.nv ? first[(size_t)w.b * a.D + w.ch + i] : 0.f;
+  if (n == 0) return;
+  const int per = (n + W - 1) / W, beg = min(n, wid * per), end = min(n, beg + per);
   const long step = (long)ds * a.B * a.D * 2;
-  const float* p = a.sum + (((size_t)s0 * a.B + w.b) * a.D + w.ch) * 2;
-  for (int k = 0; k < n; k += 8) {
+  const float* p = a.sum + (((size_t)s0 * a.B + w.b) * a.D + w.ch) * 2 + beg * step;
+  float A[VEC], H[VEC];
+#pragma unroll
+  for (int i = 0; i < VEC; ++i) {
+    A[i] = 1.f;
+    H[i] = 0.f;
+  }
+  for (int k = beg; k < end; k += 8) {
     float m[8][2 * VEC];
 #pragma unroll
     for (int j = 0; j < 8; ++j)
 #pragma unroll
-      for (int i = 0; i < 2 * VEC; ++i) m[j][i] = k + j < n && i < 2 * w.nv ? p[j * step + i] : (i & 1 ? 0.f : 1.f);
+      for (int i = 0; i < 2 * VEC; ++i) m[j][i] = k + j < end && i < 2 * w.nv ? p[j * step + i] : (i & 1 ? 0.f : 1.f);
 #pragma unroll
     for (int j = 0; j < 8; ++j)
 #pragma unroll
-      for (int i = 0; i < VEC; ++i) h[i] = m[j][2 * i] * h[i] + m[j][2 * i + 1];
+      for (int i = 0; i < VEC; ++i) {
+        A[i] *= m[j][2 * i];
+        H[i] = m[j][2 * i] * H[i] + m[j][2 * i + 1];
+      }
     p += 8 * step;
   }
-}
-// the state that enters segment seg: h0 through the summaries of the segments before it
-template <int VEC> __device__ __forceinline__ void entering(const ScanArgs& a, const Who& w, float* h) {
 #pragma unroll
-  for (int i = 0; i < VEC; ++i) h[i] = a.h0 && i < w.nv ? a.h0[(size_t)w.b * a.D + w.ch + i] : 0.f;
-  if (w.seg > 0) compose<VEC>(a, w, 0, 1, w.seg, h);
-}
-// ... and the gradient that enters it from behind
-template <int VEC> __device__ __forceinline__ void entering_back(const ScanArgs& a, const Who& w, float* c) {
+  for (int i = 0; i < VEC; ++i) {
+    ex[2 * wid][i][lane] = A[i];
+    ex[2 * wid + 1][i][lane] = H[i];
+  }
+  __syncthreads();
 #pragma unroll
-  for (int i = 0; i < VEC; ++i) c[i] = a.dhT && i < w.nv ? a.dhT[(size_t)w.b * a.D + w.ch + i] : 0.f;
-  if (w.seg < a.S - 1) compose<VEC>(a, w, a.S - 1, -1, a.S - 1 - w.seg, c);
+  for (int q = 0; q < W; ++q)
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) h[i] = ex[2 * q][i][lane] * h[i] + ex[2 * q + 1][i][lane];
+  __syncthreads();   // ex is the tiles' next
 }
 
 template <typename T, int VEC> using RawT = typename Raw<T, VEC>::t;
@@ -190,7 +200,7 @@ __global__ __launch_bounds__(64 * W) void scan_fwd_kernel(ScanArgs a) {
   const T *f = (const T*)a.f, *v = (const T*)a.v;
   T* y = (T*)a.y + w.b * a.ysb + w.ch;
   float h[VEC];
-  entering<VEC>(a, w, h);
+  entering<VEC, W>(a, w, a.h0, 0, 1, w.seg, &ex[0][0][0], h);
   RawT<T, VEC> fr[L], vr[L];
   load_piece<T, VEC>(w, f, a.fsb, a.fst, t0 * TL + wid * L, fr);
   load_piece<T, VEC>(w, v, a.vsb, a.vst, t0 * TL + wid * L, vr);
@@ -360,7 +370,7 @@ __global__ __launch_bounds__(64 * W) void scan_bwd_kernel(ScanArgs a) {
   T* df = (T*)a.df + w.b * a.gsb + w.ch;
   T* dv = (T*)a.dv + w.b * a.wsb + w.ch;
   float c[VEC];
-  entering_back<VEC>(a, w, c);
+  entering<VEC, W>(a, w, a.dhT, a.S - 1, -1, a.S - 1 - w.seg, &ex[0][0][0], c);
   RawT<T, VEC> fr[L], vr[L], dr[L];
   const int ub = (t1 - 1) * TL + wid * L;
   load_piece<T, VEC>(w, f, a.fsb, a.fst, ub, fr);
@@ -468,22 +478,22 @@ __global__ __launch_bounds__(256) void scan_pass_kernel(const float* in, float* 
 struct Plan {
   int W, S, tps, groups, tiles;
 };
-constexpr int kVec = 2;
-Plan scan_plan(int B, int T, int D, int dir) {
+Plan scan_plan(int dtype, int B, int T, int D, int dir) {
   const int Dh = dir == 2 ? D / 2 : D, nd = dir == 2 ? 2 : 1;
   Plan p;
-  p.groups = (Dh + 64 * kVec - 1) / (64 * kVec);
+  const int ch = 64 * (dtype == CRNN_BF16 ? vec_of<bf16>() : vec_of<float>());
+  p.groups = (Dh + ch - 1) / ch;
   const long rows = (long)p.groups * nd * B;   // workgroups without segments
   const long cu = crnn_cu_count();
-  const int wmax = rows < 4 * cu ? 8 : 4;
+  const int wmax = rows < 4 * cu ? kWmax : kWmax / 2;
   p.W = 1;
   while (p.W < wmax && T > p.W * L) p.W *= 2;
   p.tiles = (T + p.W * L - 1) / (p.W * L);
   p.S = 1;
-  if (p.W == 8 && rows < cu && p.tiles > 2) {
+  if (p.W == kWmax && rows < cu && p.tiles > 2) {
     long s = (2 * cu + rows - 1) / rows;
     if (s > p.tiles / 2) s = p.tiles / 2;
-    if (s > 64) s = 64;
+    if (s > 128) s = 128;
     p.S = (int)(s < 1 ? 1 : s);
   }
   p.tps = (p.tiles + p.S - 1) / p.S;
@@ -492,12 +502,13 @@ Plan scan_plan(int B, int T, int D, int dir) {
 }
 
 template <typename T, int W, bool BACK> int scan_go(const ScanArgs& a, hipStream_t st) {
+  constexpr int kVec = vec_of<T>();
   const int nd = a.dir == 2 ? 2 : 1;
   const long blocks = (long)a.groups * nd * a.B * a.S;
   if (blocks > 0x7fffffffL) return crnn_set_error(hipErrorInvalidValue, "gated_scan: too many rows");
   const dim3 grid((unsigned)blocks), block(64 * W);
   if (a.S > 1) {
-    if constexpr (W == 8) {   // only the widest tiles are cut into segments
+    if constexpr (W == kWmax) {   // only the widest tiles are cut into segments
       hipLaunchKernelGGL((scan_sum_kernel<T, kVec, W, BACK>), grid, block, 0, st, a);
       const int rc = (int)hipGetLastError();
       if (rc) return rc;
@@ -508,7 +519,7 @@ template <typename T, int W, bool BACK> int scan_go(const ScanArgs& a, hipStream
   return (int)hipGetLastError();
 }
 template <typename T, bool BACK> int scan_run(ScanArgs& a, hipStream_t st) {
-  const Plan p = scan_plan(a.B, a.T, a.D, a.dir);
+  const Plan p = scan_plan(sizeof(T) == 2 ? CRNN_BF16 : CRNN_F32, a.B, a.T, a.D, a.dir);
   a.Dh = a.dir == 2 ? a.D / 2 : a.D;
   a.groups = p.groups;
   a.S = p.S;
@@ -516,7 +527,7 @@ template <typename T, bool BACK> int scan_run(ScanArgs& a, hipStream_t st) {
   if (p.W == 1) return scan_go<T, 1, BACK>(a, st);
   if (p.W == 2) return scan_go<T, 2, BACK>(a, st);
   if (p.W == 4) return scan_go<T, 4, BACK>(a, st);
-  return scan_go<T, 8, BACK>(a, st);
+  return scan_go<T, kWmax, BACK>(a, st);
 }
 bool bad_shape(int dtype, int B, int T, int D, int dir) {
   return (dtype != CRNN_F32 && dtype != CRNN_BF16) || B < 0 || T < 0 || D < 0 || dir < 0 || dir > 2 || (dir == 2 && D % 2);
@@ -528,12 +539,12 @@ extern "C" {
 
 size_t crnn_gated_scan_ckpt_bytes(int dtype, int B, int T, int D, int dir) {
   if (bad_shape(dtype, B, T, D, dir) || !B || !T || !D) return 0;
-  return (size_t)B * scan_plan(B, T, D, dir).tiles * D * sizeof(float);
+  return (size_t)B * scan_plan(dtype, B, T, D, dir).tiles * D * sizeof(float);
 }
 
 size_t crnn_gated_scan_workspace(int dtype, int B, int T, int D, int dir) {
   if (bad_shape(dtype, B, T, D, dir) || !B || !T || !D) return 0;
-  const Plan p = scan_plan(B, T, D, dir);
+  const Plan p = scan_plan(dtype, B, T, D, dir);
   return p.S > 1 ? (size_t)p.S * B * D * 2 * sizeof(float) : 0;
 }
 
