@@ -136,7 +136,7 @@ _SEQ_TIMEOUT_MSG = ("persistent BiLSTM sweep timed out waiting for a co-resident
 class CRNNEngine:
     def __init__(self, params: Dict[str, torch.Tensor], buffers: Dict[str, torch.Tensor], hidden: int,
                  num_classes: int, num_rnn_layers: int = 2, dtype: torch.dtype = torch.bfloat16,
-                 enc_dim: int = 512, version_source=None):
+                 enc_dim: int = 512, version_source=None, rnn_type: str = "lstm"):
         self.p = params
         self.buf = buffers
         self.H = hidden
@@ -147,6 +147,12 @@ class CRNNEngine:
         self.has_head = "ctc_head.weight" in params
         self.nl = num_rnn_layers
         self.enc_dim = enc_dim
+        # the sequence stack: "lstm" (the reference's BiLSTM) or "glr" (crnn_hip/glr.py)
+        self.rnn_type = rnn_type
+        self.glr = None
+        if rnn_type == "glr":
+            from .glr import GLRStack
+            self.glr = GLRStack(self)
         self.dtype = dtype
         self.dt = L.dtype_code(dtype)
         any_p = next(iter(params.values()))
@@ -288,8 +294,9 @@ class CRNNEngine:
         # kernel (KH = KW = 1, perm = the gate interleave) when its 16-B source rows allow, else an
         # element gather in crnn_pack_batch (below)
         whh_names = [f"enc_rnn.{l}.rnn.weight_hh_l0{sfx}" for l in range(self.nl) for sfx in ("", "_reverse")]
-        tiled_t = H % 16 == 0 and all(self.p[n].data_ptr() % 16 == 0 for n in whh_names)
-        for l in range(self.nl if tiled_t else 0):
+        lstm = self.nl if self.rnn_type == "lstm" else 0
+        tiled_t = bool(lstm) and H % 16 == 0 and all(self.p[n].data_ptr() % 16 == 0 for n in whh_names)
+        for l in range(lstm if tiled_t else 0):
             pre = f"enc_rnn.{l}"
             whh_t = self._pbuf(pre + ".whh_t", (2, H, 4 * H), T)
             for d, sfx in enumerate(["", "_reverse"]):
@@ -303,7 +310,14 @@ class CRNNEngine:
             traw = None
         tw_tab = (traw, len(jobs), tiles)
         jobs.clear()
-        for l in range(self.nl):
+        if self.rnn_type == "glr":
+            from .glr import linears
+            for l in range(self.nl):
+                for name, n, k in linears(self, l):
+                    key = f"enc_rnn.{l}.{name}"
+                    w = self._pbuf(key, (n, k), T)
+                    sizes.append(job(L.PACK_ROWS, self.p[key + ".weight"], w, n, n, k))
+        for l in range(lstm):
             pre = f"enc_rnn.{l}"
             ind = self.enc_dim if l == 0 else H
             wih = self._pbuf(pre + ".wih", (2, 4 * H, ind), T)
@@ -783,6 +797,8 @@ class CRNNEngine:
     def _rnn_forward(self, seq, B, Tn, save_for_backward):
         """the BiLSTM stack (model/model.py:151-163, 195-198) over seq [B, T, enc_dim] (compute dtype)
         -> (output [B, T, hidden], per-layer saved tensors)"""
+        if self.glr is not None:
+            return self.glr.forward(seq, B, Tn, save_for_backward)
         ws, dt, T, s = self.ws, self.dt, self.dtype, L.stream_ptr()
         Hd = self.H
         xin = seq
@@ -818,7 +834,7 @@ class CRNNEngine:
         return xin, rnn_saved
 
     def bilstm_stack(self, seq: torch.Tensor, dout: Optional[torch.Tensor] = None, grads=None):
-        """The BiLSTM stack alone (model/model.py:195-198) on seq [B, T, enc_dim] fp32: -> output
+        """The sequence stack alone (model/model.py:195-198; rnn_type "glr": crnn_hip/glr.py) on seq [B, T, enc_dim] fp32: -> output
         [B, T, hidden] fp32; with dout (d loss / d output, fp32) also the BiLSTM parameter gradients
         into `grads` (overwritten) and -> (output, d seq fp32). The same kernels and workspace as the
         full forward / backward (tests: the 4 x 768 stack golden, tests/golden/bilstm_stack.npz)."""
@@ -1085,6 +1101,8 @@ class CRNNEngine:
     def _rnn_backward(self, dx, rnn_saved, B, Tn, acc):
         """BPTT through the BiLSTM stack: d output [B, T, hidden] -> d input [B, T, enc_dim]; the
         parameter gradients straight into self.g (reference layouts)"""
+        if self.glr is not None:
+            return self.glr.backward(dx, rnn_saved, B, Tn, acc)
         ws, dt, T, s = self.ws, self.dt, self.dtype, L.stream_ptr()
         Hd = self.H
         M = B * Tn

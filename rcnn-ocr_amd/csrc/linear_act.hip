@@ -84,13 +84,14 @@ template <typename T, int ACT, bool OWN = false> struct ActEpi {
   const void* bias;
   long ldy, ldz, ldr;
   int M, N, bias_f32;
-  int vec;   // y, z, res, bias aligned for 16-byte vectors
+  int vec;   // y, z, res aligned for 16-byte vectors
   __device__ __forceinline__ float b(int n) const { return bias_f32 ? ((const float*)bias)[n] : tof(((const T*)bias)[n]); }
-  __device__ __forceinline__ f32x4 b4(int n) const { return bias_f32 ? ld4f<float>((const float*)bias + n) : ld4f<T>((const T*)bias + n); }
   __device__ __forceinline__ void store(int m, int n, f32x4 v, int) const {
     if (m >= M || n >= N) return;
     if (vec && n + 4 <= N) {
-      if (bias) v += b4(n);
+      if (bias)   // element by element: a view into a flat parameter buffer is aligned to its own type only
+#pragma unroll
+        for (int r = 0; r < 4; ++r) v[r] += b(n + r);
       if (z) st4<T>(z + m * ldz + n, v);
 #pragma unroll
       for (int r = 0; r < 4; ++r) v[r] = act<T, ACT>(v[r]);
@@ -275,7 +276,7 @@ int fwd_act(const T* x, long ldx, const T* w, long ldw, const void* bias, int bi
   const long step = max_rows(ldx, sizeof(T));
   const long m16 = 16 / sizeof(T);   // elements of a 16-byte vector
   const bool al = aligned16(y) && ldy % m16 == 0 && (!z || (aligned16(z) && ldz % m16 == 0)) &&
-                  (!res || (aligned16(res) && ldr % m16 == 0)) && (!bias || aligned16(bias));
+                  (!res || (aligned16(res) && ldr % m16 == 0));
   for (long m0 = 0; m0 < M; m0 += step) {
     const int m = (int)(M - m0 < step ? M - m0 : step);
     const RowMajorK<T> la{x + m0 * ldx, (int)ldx, m, K8};

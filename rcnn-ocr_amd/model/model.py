@@ -3,7 +3,7 @@ running SE-ResNet31 -> BiLSTM -> CTC head on the MI355X HIP engine.
 
     RCNN(num_classes, hidden_size=256, sos_id=1, eos_id=2, pad_id=0, blank_id=3,
          enc_dropout_p=0.1, dropblock_p=0.0, dropblock_block_size=5,
-         decoder="ctc", num_rnn_layers=2, compute_dtype=torch.bfloat16)
+         decoder="ctc", num_rnn_layers=2, compute_dtype=torch.bfloat16, rnn_type="lstm")
     .encode(x [B,3,H,W]) -> [B, T=W/8, hidden]        (model/model.py:215-221)
     .forward(x, text=None, is_train=True, batch_max_length=25) -> CTC logits [B, T, C]
 
@@ -11,6 +11,7 @@ State-dict keys are the reference's (cnn.*, enc_rnn.*) plus ctc_head.{weight,bia
 decoder="ctc" (the reference's training head is an attention decoder; this path is
 CTC), or plus the reference's attn.* for decoder="attn" — exactly the reference's key set, so its
 checkpoints load strictly.
+rnn_type="glr" puts the gated-linear-recurrence stack (crnn_hip/glr.py) in the BiLSTM's place, with its own enc_rnn.* keys.
 Every forward/backward runs in libcrnn_hip.so; there is no CPU path — on a CPU
 tensor the module raises.
 """
@@ -38,6 +39,28 @@ class BidirectionalLSTM(nn.Module):
 
     def forward(self, x):
         raise NotImplementedError("BiLSTM layers run inside the HIP engine; call RCNN.encode/forward")
+
+
+class GatedLinearLayer(nn.Module):
+    """parameter container of one gated-linear-recurrence layer (crnn_hip/glr.py): pre-norm, gate logits and values of both
+    directions in one projection, output projection; pre-norm, two-layer feed-forward. proj: only where the input's width
+    differs. Gates start biased to remember (sigmoid(1) = 0.73)."""
+
+    def __init__(self, input_size, hidden_size):
+        super().__init__()
+        if input_size != hidden_size:
+            self.proj = nn.Linear(input_size, hidden_size)
+        self.norm1 = nn.LayerNorm(hidden_size)
+        self.add_module("in", nn.Linear(hidden_size, 4 * hidden_size))
+        self.out = nn.Linear(2 * hidden_size, hidden_size)
+        self.norm2 = nn.LayerNorm(hidden_size)
+        self.ff1 = nn.Linear(hidden_size, 2 * hidden_size)
+        self.ff2 = nn.Linear(2 * hidden_size, hidden_size)
+        with torch.no_grad():
+            getattr(self, "in").bias[: 2 * hidden_size] += 1.0
+
+    def forward(self, x):
+        raise NotImplementedError("sequence layers run inside the HIP engine; call RCNN.encode/forward")
 
 
 def _noop():
@@ -131,22 +154,28 @@ class RCNN(nn.Module):
     def __init__(self, num_classes, hidden_size=256, sos_id: int = 1, eos_id: int = 2, pad_id: int = 0,
                  blank_id: Optional[int] = 3, enc_dropout_p: float = 0.1, dropblock_p: float = 0.0,
                  dropblock_block_size: int = 5, decoder: str = "ctc", num_rnn_layers: int = 2,
-                 compute_dtype: torch.dtype = torch.bfloat16):
+                 compute_dtype: torch.dtype = torch.bfloat16, rnn_type: str = "lstm"):
         super().__init__()
         if decoder not in ("ctc", "attn"):
             raise ValueError(f"decoder must be 'ctc' or 'attn', got {decoder!r}")
+        if rnn_type not in ("lstm", "glr"):
+            raise ValueError(f"rnn_type must be 'lstm' or 'glr', got {rnn_type!r}")
         self.num_classes = num_classes
         self.hidden_size = hidden_size
         self.sos_id, self.eos_id, self.pad_id, self.blank_id = sos_id, eos_id, pad_id, blank_id
         self.decoder = decoder
         self.num_rnn_layers = num_rnn_layers
         self.compute_dtype = compute_dtype
+        self.rnn_type = rnn_type
         self.cnn = SEResNet31(in_channels=3, out_channels=512, dropblock_p=dropblock_p,
                               dropblock_block_size=dropblock_block_size)
         self.pool = nn.AdaptiveAvgPool2d((1, None))
         enc_dim = self.cnn.out_channels
-        layers = [BidirectionalLSTM(enc_dim, hidden_size, hidden_size)]
-        layers += [BidirectionalLSTM(hidden_size, hidden_size, hidden_size) for _ in range(1, num_rnn_layers)]
+        widths = [enc_dim] + [hidden_size] * (num_rnn_layers - 1)
+        if rnn_type == "lstm":
+            layers = [BidirectionalLSTM(w, hidden_size, hidden_size) for w in widths]
+        else:
+            layers = [GatedLinearLayer(w, hidden_size) for w in widths]
         self.enc_rnn = nn.Sequential(*layers)
         self.enc_dropout = nn.Dropout(enc_dropout_p)
         self.ctc_head = nn.Linear(hidden_size, num_classes) if decoder == "ctc" else None
@@ -253,7 +282,7 @@ class RCNN(nn.Module):
             self.flatten_parameters_()
             self._engine = CRNNEngine(self._param_dict(), self._buffer_dict(), self.hidden_size,
                                       self.num_classes, self.num_rnn_layers, self.compute_dtype,
-                                      version_source=self._param_version)
+                                      version_source=self._param_version, rnn_type=self.rnn_type)
         return self._engine
 
     def _param_version(self) -> int:

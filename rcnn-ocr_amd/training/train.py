@@ -13,7 +13,7 @@ evaluation, resume from a checkpoint, and the scheduler step rules.
 
 New keys of this path (SURVEY §5 "Config"): `decoder` ("ctc", this path's default: CTC head +
 CTC loss; "attn": the reference's attention head + cross-entropy), `num_rnn_layers`
-(2), `dtype` ("bf16" | "fp32"), `enc_dropout_p` (0.1), `world_size` (data parallel).
+(2), `rnn_type` ("lstm", the reference's BiLSTM; "glr": the gated-linear-recurrence stack), `dtype` ("bf16" | "fp32"), `enc_dropout_p` (0.1), `world_size` (data parallel).
 
 Data parallel (`world_size` > 1, one process per GPU under `torchrun --nproc-per-node N`): every
 rank builds the same model and takes rank 0's weights (broadcast of the flat parameter buffer);
@@ -317,6 +317,7 @@ def run_training(cfg: Config, device: str = "cuda") -> Dict[str, object]:
     val_size = getattr(cfg, "val_size", 3000)
     decoder = getattr(cfg, "decoder", "ctc")
     num_rnn_layers = getattr(cfg, "num_rnn_layers", 2)
+    rnn_type = getattr(cfg, "rnn_type", "lstm")
     dtype = {"bf16": torch.bfloat16, "fp32": torch.float32}[getattr(cfg, "dtype", "bf16")]
     enc_dropout_p = getattr(cfg, "enc_dropout_p", 0.1)
 
@@ -341,7 +342,7 @@ def run_training(cfg: Config, device: str = "cuda") -> Dict[str, object]:
     logger.info(f"Charset loaded: {len(itos)} tokens")
     model = RCNN(num_classes=len(itos), hidden_size=hidden_size, sos_id=SOS, eos_id=EOS, pad_id=PAD, blank_id=BLANK,
                  enc_dropout_p=enc_dropout_p, decoder=decoder, num_rnn_layers=num_rnn_layers,
-                 compute_dtype=dtype).to(dev)
+                 compute_dtype=dtype, rnn_type=rnn_type).to(dev)
     reducer = None
     if world > 1:
         from crnn_hip import dist as D
@@ -435,7 +436,8 @@ def run_training(cfg: Config, device: str = "cuda") -> Dict[str, object]:
                  "img_w": img_w, "encoding": encoding, "max_len": max_len, "charset_path": charset_path,
                  "train_csvs": cfg.train_csvs, "train_roots": cfg.train_roots,
                  "val_csvs": getattr(cfg, "val_csvs", None), "val_roots": getattr(cfg, "val_roots", None),
-                 "hidden_size": hidden_size, "decoder": decoder, "num_rnn_layers": num_rnn_layers}
+                 "hidden_size": hidden_size, "decoder": decoder, "num_rnn_layers": num_rnn_layers,
+                 "rnn_type": rnn_type}
 
     def deal(items):
         """this rank's share: every world-th item from its rank, the same count on every rank"""

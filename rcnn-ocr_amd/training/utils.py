@@ -67,9 +67,13 @@ def rcnn_from_state(model_state, num_classes, hidden_size, sos_id, eos_id, pad_i
         decoder = "attn"
     else:
         raise ValueError("checkpoint has neither ctc_head.* nor attn.* weights: no decoder to load")
-    n_rnn = len({k.split(".")[1] for k in model_state if k.startswith("enc_rnn.") and k.endswith("linear.bias")})
+    # a BiLSTM layer ends in linear.*, a gated-linear-recurrence layer in ff2.*
+    rnn_type = "glr" if any(k.startswith("enc_rnn.") and k.endswith(".ff2.bias") for k in model_state) else "lstm"
+    last = ".ff2.bias" if rnn_type == "glr" else "linear.bias"
+    n_rnn = len({k.split(".")[1] for k in model_state if k.startswith("enc_rnn.") and k.endswith(last)})
     model = RCNN(num_classes=num_classes, hidden_size=hidden_size, sos_id=sos_id, eos_id=eos_id, pad_id=pad_id,
-                 blank_id=blank_id, decoder=decoder, num_rnn_layers=max(1, n_rnn), compute_dtype=compute_dtype)
+                 blank_id=blank_id, decoder=decoder, num_rnn_layers=max(1, n_rnn), compute_dtype=compute_dtype,
+                 rnn_type=rnn_type)
     model.load_state_dict(model_state, strict=True)
     return model
 
