@@ -42,10 +42,12 @@ template <typename T, int VEC> __device__ __forceinline__ void set_elem(typename
   if constexpr (sizeof(T) == 2) r[i] = __builtin_bit_cast(unsigned short, (bf16)v);
   else r[i] = v;
 }
-// nv: this lane's channels that exist (0 .. VEC)
-template <typename T, int VEC> __device__ __forceinline__ typename Raw<T, VEC>::t ldv(const T* p, int nv) {
+// nv: this lane's channels that exist (0 .. VEC); FULL: all of them in every lane of the wave, which spares each access its
+// branch, as whole pieces within the length do (2 x 16384 x 1024 bf16, forward / backward with all of them: 70 / 99 us,
+// without 57 / 89; 256 x 32 x 1024 both ways: 13.2 / 19.9, 10.7 / 17.4)
+template <typename T, int VEC, bool FULL> __device__ __forceinline__ typename Raw<T, VEC>::t ldv(const T* p, int nv) {
   typename Raw<T, VEC>::t r = {};
-  if (nv == VEC) {
+  if (FULL || nv == VEC) {
     r = *reinterpret_cast<const typename RawU<T, VEC>::t*>(p);
   } else {
 #pragma unroll
@@ -54,8 +56,8 @@ template <typename T, int VEC> __device__ __forceinline__ typename Raw<T, VEC>::
   }
   return r;
 }
-template <typename T, int VEC> __device__ __forceinline__ void stv(T* p, int nv, const float* v) {
-  if (nv == VEC) {
+template <typename T, int VEC, bool FULL> __device__ __forceinline__ void stv(T* p, int nv, const float* v) {
+  if (FULL || nv == VEC) {
     typename Raw<T, VEC>::t r = {};
 #pragma unroll
     for (int i = 0; i < VEC; ++i) set_elem<T, VEC>(r, i, v[i]);
@@ -172,46 +174,62 @@ __device__ __forceinline__ void entering(const ScanArgs& a, const Who& w, const 
 template <typename T, int VEC> using RawT = typename Raw<T, VEC>::t;
 
 // the L steps from walking step u0 of one tensor (nothing is read at or behind the length)
-template <typename T, int VEC>
+template <typename T, int VEC, bool FULL>
 __device__ __forceinline__ void load_piece(const Who& w, const T* p, long sb, long st, int u0, RawT<T, VEC>* r) {
   const T* base = p + w.b * sb + w.ch;
   if (u0 + L <= w.len) {
     const long step = w.rev ? -st : st;
     base += at(w, u0) * st;
 #pragma unroll
-    for (int i = 0; i < L; ++i) r[i] = ldv<T, VEC>(base + i * step, w.nv);
+    for (int i = 0; i < L; ++i) r[i] = ldv<T, VEC, FULL>(base + i * step, w.nv);
   } else {
 #pragma unroll
     for (int i = 0; i < L; ++i) {
       RawT<T, VEC> z = {};
       r[i] = z;
-      if (u0 + i < w.len) r[i] = ldv<T, VEC>(base + at(w, u0 + i) * st, w.nv);
+      if (u0 + i < w.len) r[i] = ldv<T, VEC, FULL>(base + at(w, u0 + i) * st, w.nv);
     }
   }
 }
+// the same steps' results; zero at and behind the length, nothing at or behind T
+template <typename T, int VEC, bool FULL>
+__device__ __forceinline__ void store_piece(const Who& w, int T_, T* p, long sb, long st, int u0, const float (*v)[VEC]) {
+  T* base = p + w.b * sb + w.ch;
+  if (u0 + L <= w.len) {
+    const long step = w.rev ? -st : st;
+    base += at(w, u0) * st;
+#pragma unroll
+    for (int i = 0; i < L; ++i) stv<T, VEC, FULL>(base + i * step, w.nv, v[i]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < L; ++i) {
+      if (u0 + i >= T_) break;
+      float o[VEC];
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) o[e] = u0 + i < w.len ? v[i][e] : 0.f;
+      stv<T, VEC, FULL>(base + at(w, u0 + i) * st, w.nv, o);
+    }
+  }
+}
+// every lane of the wave has all its channels
+template <int VEC> __device__ __forceinline__ bool full_wave(const ScanArgs& a) {
+  return (int)(blockIdx.x % a.groups + 1) * 64 * VEC <= a.Dh;
+}
 
-template <typename T, int VEC, int W>
-__global__ __launch_bounds__(64 * W) void scan_fwd_kernel(ScanArgs a) {
+template <typename T, int VEC, int W, bool FULL> __device__ __forceinline__ void scan_fwd(const ScanArgs& a, float (*ex)[W][2][VEC][64]) {
   constexpr int TL = W * L;
-  __shared__ float ex[2][W][2][VEC][64];
   const Who w = who<VEC>(a);
   const int lane = threadIdx.x & 63, wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int tiles = (a.T + TL - 1) / TL, t0 = w.seg * a.tps, t1 = min(tiles, t0 + a.tps);
   const T *f = (const T*)a.f, *v = (const T*)a.v;
-  T* y = (T*)a.y + w.b * a.ysb + w.ch;
   float h[VEC];
   entering<VEC, W>(a, w, a.h0, 0, 1, w.seg, &ex[0][0][0], h);
   RawT<T, VEC> fr[L], vr[L];
-  load_piece<T, VEC>(w, f, a.fsb, a.fst, t0 * TL + wid * L, fr);
-  load_piece<T, VEC>(w, v, a.vsb, a.vst, t0 * TL + wid * L, vr);
+  load_piece<T, VEC, FULL>(w, f, a.fsb, a.fst, t0 * TL + wid * L, fr);
+  load_piece<T, VEC, FULL>(w, v, a.vsb, a.vst, t0 * TL + wid * L, vr);
   for (int t = t0; t < t1; ++t) {
     const int u0 = t * TL + wid * L;
     float al[L][VEC], ul[L][VEC], A[VEC], H[VEC];
-#pragma unroll
-    for (int i = 0; i < VEC; ++i) {
-      A[i] = 1.f;
-      H[i] = 0.f;
-    }
 #pragma unroll
     for (int s = 0; s < L; ++s)
 #pragma unroll
@@ -219,21 +237,37 @@ __global__ __launch_bounds__(64 * W) void scan_fwd_kernel(ScanArgs a) {
         float r;
         gate<T>(elem<T, VEC>(fr[s], i), al[s][i], r);
         ul[s][i] = r * elem<T, VEC>(vr[s], i);
-        if (u0 + s >= w.len) {
-          al[s][i] = 1.f;
-          ul[s][i] = 0.f;
-        }
+      }
+    if (u0 + L > w.len) {
+#pragma unroll
+      for (int s = 0; s < L; ++s)
+#pragma unroll
+        for (int i = 0; i < VEC; ++i)
+          if (u0 + s >= w.len) {
+            al[s][i] = 1.f;
+            ul[s][i] = 0.f;
+          }
+    }
+    if (t + 1 < t1) {   // the next tile's piece while this one is finished
+      load_piece<T, VEC, FULL>(w, f, a.fsb, a.fst, u0 + TL, fr);
+      load_piece<T, VEC, FULL>(w, v, a.vsb, a.vst, u0 + TL, vr);
+    }
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) {
+      A[i] = al[0][i];
+      H[i] = ul[0][i];
+    }
+#pragma unroll
+    for (int s = 1; s < L; ++s)
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) {
         A[i] *= al[s][i];
         H[i] = al[s][i] * H[i] + ul[s][i];
       }
-    if (t + 1 < t1) {   // the next tile's piece while this one is finished
-      load_piece<T, VEC>(w, f, a.fsb, a.fst, u0 + TL, fr);
-      load_piece<T, VEC>(w, v, a.vsb, a.vst, u0 + TL, vr);
-    }
     if (a.ckpt && wid == 0) {
 #pragma unroll
       for (int i = 0; i < VEC; ++i)
-        if (i < w.nv) a.ckpt[((size_t)w.b * tiles + t) * a.D + w.ch + i] = h[i];
+        if (FULL || i < w.nv) a.ckpt[((size_t)w.b * tiles + t) * a.D + w.ch + i] = h[i];
     }
     float hin[VEC];
     if constexpr (W > 1) {
@@ -260,16 +294,10 @@ __global__ __launch_bounds__(64 * W) void scan_fwd_kernel(ScanArgs a) {
       }
     }
 #pragma unroll
-    for (int s = 0; s < L; ++s) {
+    for (int s = 0; s < L; ++s)
 #pragma unroll
-      for (int i = 0; i < VEC; ++i) hin[i] = al[s][i] * hin[i] + ul[s][i];
-      if (u0 + s < a.T) {
-        float o[VEC];
-#pragma unroll
-        for (int i = 0; i < VEC; ++i) o[i] = u0 + s < w.len ? hin[i] : 0.f;
-        stv<T, VEC>(y + at(w, u0 + s) * a.yst, w.nv, o);
-      }
-    }
+      for (int i = 0; i < VEC; ++i) ul[s][i] = hin[i] = al[s][i] * hin[i] + ul[s][i];
+    store_piece<T, VEC, FULL>(w, a.T, (T*)a.y, a.ysb, a.yst, u0, ul);
   }
   if (a.hT && w.seg == a.S - 1 && wid == 0) {
 #pragma unroll
@@ -277,14 +305,16 @@ __global__ __launch_bounds__(64 * W) void scan_fwd_kernel(ScanArgs a) {
       if (i < w.nv) a.hT[(size_t)w.b * a.D + w.ch + i] = h[i];
   }
 }
+template <typename T, int VEC, int W> __global__ __launch_bounds__(64 * W) void scan_fwd_kernel(ScanArgs a) {
+  __shared__ float ex[2][W][2][VEC][64];
+  if (full_wave<VEC>(a)) scan_fwd<T, VEC, W, true>(a, ex);
+  else scan_fwd<T, VEC, W, false>(a, ex);
+}
 
 // (A, H) of a segment, or (A, C) of the reverse recurrence (BACK): each wave sums up its share of the segment, then the
 // shares are joined in order
-template <typename T, int VEC, int W, bool BACK>
-__global__ __launch_bounds__(64 * W) void scan_sum_kernel(ScanArgs a) {
-  __shared__ float ex[W][2][VEC][64];
+template <typename T, int VEC, int W, bool BACK, bool FULL> __device__ __forceinline__ void scan_sum(const ScanArgs& a, float (*ex)[2][VEC][64]) {
   const Who w = who<VEC>(a);
-  if (w.seg == (BACK ? 0 : a.S - 1)) return;   // nobody comes after it
   const int lane = threadIdx.x & 63, wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int per = a.tps * L, beg = w.seg * a.tps * W * L + wid * per;   // this wave's steps [beg, beg + per)
   const T *f = (const T*)a.f, *q = BACK ? (const T*)a.dy : (const T*)a.v;
@@ -297,8 +327,8 @@ __global__ __launch_bounds__(64 * W) void scan_sum_kernel(ScanArgs a) {
   }
   RawT<T, VEC> fr[L], qr[L];
   const int first = BACK ? beg + per - L : beg;
-  load_piece<T, VEC>(w, f, a.fsb, a.fst, first, fr);
-  load_piece<T, VEC>(w, q, qsb, qst, first, qr);
+  load_piece<T, VEC, FULL>(w, f, a.fsb, a.fst, first, fr);
+  load_piece<T, VEC, FULL>(w, q, qsb, qst, first, qr);
   for (int k = 0; k < a.tps; ++k) {
     const int u0 = BACK ? first - k * L : first + k * L;
     float al[L][VEC], ul[L][VEC];
@@ -309,14 +339,20 @@ __global__ __launch_bounds__(64 * W) void scan_sum_kernel(ScanArgs a) {
         float r;
         gate<T>(elem<T, VEC>(fr[s], i), al[s][i], r);
         ul[s][i] = BACK ? elem<T, VEC>(qr[s], i) : r * elem<T, VEC>(qr[s], i);
-        if (u0 + s >= w.len) {
-          al[s][i] = 1.f;
-          ul[s][i] = 0.f;
-        }
       }
+    if (u0 + L > w.len) {
+#pragma unroll
+      for (int s = 0; s < L; ++s)
+#pragma unroll
+        for (int i = 0; i < VEC; ++i)
+          if (u0 + s >= w.len) {
+            al[s][i] = 1.f;
+            ul[s][i] = 0.f;
+          }
+    }
     if (k + 1 < a.tps) {
-      load_piece<T, VEC>(w, f, a.fsb, a.fst, BACK ? u0 - L : u0 + L, fr);
-      load_piece<T, VEC>(w, q, qsb, qst, BACK ? u0 - L : u0 + L, qr);
+      load_piece<T, VEC, FULL>(w, f, a.fsb, a.fst, BACK ? u0 - L : u0 + L, fr);
+      load_piece<T, VEC, FULL>(w, q, qsb, qst, BACK ? u0 - L : u0 + L, qr);
     }
 #pragma unroll
     for (int s = 0; s < L; ++s)
@@ -359,29 +395,32 @@ __global__ __launch_bounds__(64 * W) void scan_sum_kernel(ScanArgs a) {
   }
 }
 
-template <typename T, int VEC, int W>
-__global__ __launch_bounds__(64 * W) void scan_bwd_kernel(ScanArgs a) {
+template <typename T, int VEC, int W, bool BACK> __global__ __launch_bounds__(64 * W) void scan_sum_kernel(ScanArgs a) {
+  __shared__ float ex[W][2][VEC][64];
+  if (who<VEC>(a).seg == (BACK ? 0 : a.S - 1)) return;   // nobody comes after it
+  if (full_wave<VEC>(a)) scan_sum<T, VEC, W, BACK, true>(a, ex);
+  else scan_sum<T, VEC, W, BACK, false>(a, ex);
+}
+
+template <typename T, int VEC, int W, bool FULL> __device__ __forceinline__ void scan_bwd(const ScanArgs& a, float (*ex)[W][3][VEC][64]) {
   constexpr int TL = W * L;
-  __shared__ float ex[2][W][3][VEC][64];
   const Who w = who<VEC>(a);
   const int lane = threadIdx.x & 63, wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int tiles = (a.T + TL - 1) / TL, t0 = w.seg * a.tps, t1 = min(tiles, t0 + a.tps);
   const T *f = (const T*)a.f, *v = (const T*)a.v, *dy = (const T*)a.dy;
-  T* df = (T*)a.df + w.b * a.gsb + w.ch;
-  T* dv = (T*)a.dv + w.b * a.wsb + w.ch;
   float c[VEC];
   entering<VEC, W>(a, w, a.dhT, a.S - 1, -1, a.S - 1 - w.seg, &ex[0][0][0], c);
   RawT<T, VEC> fr[L], vr[L], dr[L];
   const int ub = (t1 - 1) * TL + wid * L;
-  load_piece<T, VEC>(w, f, a.fsb, a.fst, ub, fr);
-  load_piece<T, VEC>(w, v, a.vsb, a.vst, ub, vr);
-  load_piece<T, VEC>(w, dy, a.dsb, a.dst, ub, dr);
+  load_piece<T, VEC, FULL>(w, f, a.fsb, a.fst, ub, fr);
+  load_piece<T, VEC, FULL>(w, v, a.vsb, a.vst, ub, vr);
+  load_piece<T, VEC, FULL>(w, dy, a.dsb, a.dst, ub, dr);
   for (int t = t1 - 1; t >= t0; --t) {
     const int u0 = t * TL + wid * L;
     float al[L][VEC], rl[L][VEC], vl[L][VEC], dl[L][VEC], A[VEC], H[VEC], C[VEC], hin[VEC];
 #pragma unroll
     for (int i = 0; i < VEC; ++i) {
-      hin[i] = i < w.nv ? a.ckpt[((size_t)w.b * tiles + t) * a.D + w.ch + i] : 0.f;
+      hin[i] = FULL || i < w.nv ? a.ckpt[((size_t)w.b * tiles + t) * a.D + w.ch + i] : 0.f;
       A[i] = 1.f;
       H[i] = C[i] = 0.f;
     }
@@ -392,10 +431,21 @@ __global__ __launch_bounds__(64 * W) void scan_bwd_kernel(ScanArgs a) {
         gate<T>(elem<T, VEC>(fr[s], i), al[s][i], rl[s][i]);
         vl[s][i] = elem<T, VEC>(vr[s], i);
         dl[s][i] = elem<T, VEC>(dr[s], i);
-        if (u0 + s >= w.len) {
-          al[s][i] = 1.f;
-          rl[s][i] = vl[s][i] = dl[s][i] = 0.f;
-        }
+      }
+    if (u0 + L > w.len) {
+#pragma unroll
+      for (int s = 0; s < L; ++s)
+#pragma unroll
+        for (int i = 0; i < VEC; ++i)
+          if (u0 + s >= w.len) {
+            al[s][i] = 1.f;
+            rl[s][i] = vl[s][i] = dl[s][i] = 0.f;
+          }
+    }
+#pragma unroll
+    for (int s = 0; s < L; ++s)
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) {
         A[i] *= al[s][i];
         H[i] = al[s][i] * H[i] + rl[s][i] * vl[s][i];
       }
@@ -404,9 +454,9 @@ __global__ __launch_bounds__(64 * W) void scan_bwd_kernel(ScanArgs a) {
 #pragma unroll
       for (int i = 0; i < VEC; ++i) C[i] = al[s][i] * (dl[s][i] + C[i]);
     if (t > t0) {
-      load_piece<T, VEC>(w, f, a.fsb, a.fst, u0 - TL, fr);
-      load_piece<T, VEC>(w, v, a.vsb, a.vst, u0 - TL, vr);
-      load_piece<T, VEC>(w, dy, a.dsb, a.dst, u0 - TL, dr);
+      load_piece<T, VEC, FULL>(w, f, a.fsb, a.fst, u0 - TL, fr);
+      load_piece<T, VEC, FULL>(w, v, a.vsb, a.vst, u0 - TL, vr);
+      load_piece<T, VEC, FULL>(w, dy, a.dsb, a.dst, u0 - TL, dr);
     }
     float cin[VEC];
     if constexpr (W > 1) {
@@ -445,28 +495,27 @@ __global__ __launch_bounds__(64 * W) void scan_bwd_kernel(ScanArgs a) {
         hin[i] = al[s][i] * hin[i] + rl[s][i] * vl[s][i];
       }
 #pragma unroll
-    for (int s = L - 1; s >= 0; --s) {
-      float gf[VEC], gv[VEC];
+    for (int s = L - 1; s >= 0; --s)
 #pragma unroll
       for (int i = 0; i < VEC; ++i) {
-        const float g = dl[s][i] + cin[i];
-        gv[i] = g * rl[s][i];
-        gf[i] = gv[i] * al[s][i] * (hp[s][i] - vl[s][i]);
+        const float g = dl[s][i] + cin[i], gv = g * rl[s][i];
         cin[i] = al[s][i] * g;
-        if (u0 + s >= w.len) gf[i] = gv[i] = 0.f;
+        dl[s][i] = gv * al[s][i] * (hp[s][i] - vl[s][i]);
+        rl[s][i] = gv;
       }
-      if (u0 + s < a.T) {
-        const int tt = at(w, u0 + s);
-        stv<T, VEC>(df + tt * a.gst, w.nv, gf);
-        stv<T, VEC>(dv + tt * a.wst, w.nv, gv);
-      }
-    }
+    store_piece<T, VEC, FULL>(w, a.T, (T*)a.df, a.gsb, a.gst, u0, dl);
+    store_piece<T, VEC, FULL>(w, a.T, (T*)a.dv, a.wsb, a.wst, u0, rl);
   }
   if (a.dh0 && w.seg == 0 && wid == 0) {
 #pragma unroll
     for (int i = 0; i < VEC; ++i)
       if (i < w.nv) a.dh0[(size_t)w.b * a.D + w.ch + i] = c[i];
   }
+}
+template <typename T, int VEC, int W> __global__ __launch_bounds__(64 * W) void scan_bwd_kernel(ScanArgs a) {
+  __shared__ float ex[2][W][3][VEC][64];
+  if (full_wave<VEC>(a)) scan_bwd<T, VEC, W, true>(a, ex);
+  else scan_bwd<T, VEC, W, false>(a, ex);
 }
 
 // T = 0: no steps, the state passes through
