@@ -557,7 +557,7 @@ long crnn_preprocess_workspace(int B, int H, int W);
 /* ------------------------------------------------------------------ layer norm
  * y[m][n] = (x[m][n] - mean_m) * rstd_m * w[n] + b[n] over the last axis, rstd = 1 / sqrt(var + eps), var the population
  * variance. x, y in dtype (fp32 or bf16) with row strides ldx, ldy >= N; w, b fp32 (either may be NULL: 1, 0);
- * mean, rstd [M] fp32 outputs for the backward (both NULL: inference). Any M >= 0, N >= 1, any alignment of the
+ * mean, rstd [M] fp32 outputs for the backward (both NULL: inference). Any M >= 0, 1 <= N <= 2^30, any alignment of the
  * elements' own type. */
 int crnn_layernorm_fwd(int dtype, const void* x, long ldx, const float* w, const float* b, void* y, long ldy, float* mean,
                        float* rstd, long M, int N, float eps, void* stream);
@@ -575,7 +575,7 @@ int crnn_layernorm_bwd(int dtype, const void* dy, long lddy, const void* x, long
  * residual in fp32, one rounding. x, w, y, res in dtype; bias fp32 (bias_f32 = 1) or dtype; bias, res may be NULL.
  * z (NULL: not stored) = the pre-activation in dtype, which the backward of gelu / silu / relu reads.
  * Any M >= 0, N, K >= 1 and element-aligned row strides: operands whose rows are not 16-byte aligned multiples of 8
- * are first copied into ws (crnn_linear_fwd_workspace bytes, 0 for aligned ones). w stays under 2 GiB. */
+ * are first copied into ws (crnn_linear_fwd_workspace bytes; 0 for aligned ones and for up to 32 rows). w stays under 2 GiB. */
 #define CRNN_ACT_NONE 0
 #define CRNN_ACT_RELU 1
 #define CRNN_ACT_GELU 2 /* z Phi(z), the erf form */

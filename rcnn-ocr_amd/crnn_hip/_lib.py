@@ -280,13 +280,16 @@ def call_on(t: torch.Tensor, name: str, *args):
 
 
 def rows(t: torch.Tensor):
-    """t [..., N] as M rows of N contiguous elements -> (tensor, M, row stride): t itself where its strides allow, else a
-    contiguous copy"""
+    """t [..., N] as M rows of N contiguous elements -> (tensor, M, row stride): t itself where its strides allow (rows one
+    constant stride >= N apart), else a contiguous copy"""
     n = t.shape[-1]
     if t.is_contiguous():
         return t, t.numel() // n if n else 0, n
-    if t.dim() == 2 and (t.stride(1) == 1 or n == 1) and t.stride(0) >= n:
-        return t, t.shape[0], t.stride(0)
+    if t.dim() >= 2 and (t.stride(-1) == 1 or n == 1):
+        size, stride = t.shape[:-1], t.stride()[:-1]
+        ld = stride[-1]
+        if ld >= n and all(stride[i] == stride[i + 1] * size[i + 1] for i in range(len(size) - 1)):
+            return t, t.numel() // n, ld
     return t.contiguous(), t.numel() // n if n else 0, n
 
 
@@ -301,6 +304,12 @@ def check_operand(op: str, name: str, t, shape, dtype, device):
         raise ValueError(f"{op}: {name} must be {' or '.join(str(d) for d in ok)}, got {t.dtype}")
     if t.device != device:
         raise ValueError(f"{op}: {name} must be on {device}, got {t.device}")
+
+
+def check_sizes(op: str, *sizes):
+    """the C ABI's sizes are ints"""
+    if max(sizes) >= 1 << 31:
+        raise ValueError(f"{op}: sizes must be below 2^31, got {sizes}")
 
 
 def differentiable_once(backward):

@@ -87,6 +87,7 @@ def linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] =
     if weight.dim() != 2 or weight.shape[1] != x.shape[-1] or weight.shape[0] < 1 or weight.shape[1] < 1:
         raise ValueError(f"linear: weight must be [N, {x.shape[-1]}] with N, K >= 1, got {tuple(weight.shape)}")
     n = weight.shape[0]
+    L.check_sizes("linear", *weight.shape)
     if bias is not None:
         L.check_operand("linear", "bias", bias, (n,), (x.dtype, torch.float32), x.device)
         bias = bias.contiguous()

@@ -57,6 +57,8 @@ def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Opt
     if x.dim() < 1 or x.shape[-1] < 1:
         raise ValueError(f"layer_norm: x needs a last axis of at least one element, got {tuple(x.shape)}")
     n = x.shape[-1]
+    if n > 1 << 30:
+        raise ValueError(f"layer_norm: the last axis must be at most 2^30, got {n}")
     if weight is not None:
         L.check_operand("layer_norm", "weight", weight, (n,), torch.float32, x.device)
         weight = weight.contiguous()

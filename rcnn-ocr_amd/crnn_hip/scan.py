@@ -96,6 +96,7 @@ def gated_scan(f: torch.Tensor, v: torch.Tensor, h0: Optional[torch.Tensor] = No
         raise ValueError(f"gated_scan: f must be [B, T, D], got {tuple(f.shape)}")
     L.check_operand("gated_scan", "v", v, f.shape, f.dtype, f.device)
     B, T, D = f.shape
+    L.check_sizes("gated_scan", B, T, D)
     if dr == 2 and D % 2:
         raise ValueError(f"gated_scan: direction 'both' needs an even number of channels, got {D}")
     if h0 is not None:
@@ -122,6 +123,7 @@ def gated_scan_step(f: torch.Tensor, v: torch.Tensor, state: torch.Tensor, out_s
     L.dtype_code(f.dtype)
     if f.dim() != 2:
         raise ValueError(f"gated_scan_step: f must be [B, D], got {tuple(f.shape)}")
+    L.check_sizes("gated_scan_step", *f.shape)
     L.check_operand("gated_scan_step", "v", v, f.shape, f.dtype, f.device)
     L.check_operand("gated_scan_step", "state", state, f.shape, torch.float32, f.device)
     if torch.is_grad_enabled() and (f.requires_grad or v.requires_grad or state.requires_grad):

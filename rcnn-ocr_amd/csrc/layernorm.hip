@@ -447,6 +447,8 @@ LnPlan ln_plan(int N) {
   return {0, 0};
 }
 
+constexpr int kMaxN = 1 << 30;   // column counters are 32 bits
+
 // workgroups of the backward: enough rows in flight, few partial rows to add up, and two rows a wave or more so that the
 // next one's loads run under this one's sums (65536 x 768 bf16, backward: 85 us at 2 workgroups per CU, 66 at 3, 88 at 4;
 // 32768 x 1536, 4 waves a row and fewer registers: 91, 67, 62; 1999 x 1021 fp32: 14.8 at one row a wave, 13.4 at two, 15.9 at
@@ -536,7 +538,8 @@ extern "C" {
 int crnn_layernorm_fwd(int dtype, const void* x, long ldx, const float* w, const float* b, void* y, long ldy, float* mean,
                        float* rstd, long M, int N, float eps, void* stream) {
   if (dtype != CRNN_F32 && dtype != CRNN_BF16) return crnn_set_error(hipErrorInvalidValue, "layernorm_fwd: dtype fp32 or bf16");
-  if (M < 0 || N < 1 || ldx < N || ldy < N) return crnn_set_error(hipErrorInvalidValue, "layernorm_fwd: M >= 0, N >= 1, ld >= N");
+  if (M < 0 || N < 1 || N > kMaxN || ldx < N || ldy < N)
+    return crnn_set_error(hipErrorInvalidValue, "layernorm_fwd: M >= 0, 1 <= N <= 2^30, ld >= N");
   if ((mean == nullptr) != (rstd == nullptr)) return crnn_set_error(hipErrorInvalidValue, "layernorm_fwd: mean and rstd go together");
   if (M == 0) return 0;
   if (!x || !y) return crnn_set_error(hipErrorInvalidValue, "layernorm_fwd: null x / y");
@@ -547,7 +550,7 @@ int crnn_layernorm_fwd(int dtype, const void* x, long ldx, const float* w, const
 
 size_t crnn_layernorm_bwd_workspace(int dtype, long M, int N) {
   (void)dtype;
-  if (M < 0 || N < 1) return 0;
+  if (M < 0 || N < 1 || N > kMaxN) return 0;
   const size_t g = ln_plan(N).wpr ? (size_t)ln_bwd_grid(M, N) : (size_t)ln_wide_slices(M);
   return g * 2 * (size_t)N * sizeof(float);
 }
@@ -556,8 +559,8 @@ int crnn_layernorm_bwd(int dtype, const void* dy, long lddy, const void* x, long
                        const float* rstd, const void* dres, long ldr, void* dx, long lddx, float* dw, float* db,
                        int accumulate, float* ws, size_t ws_bytes, long M, int N, void* stream) {
   if (dtype != CRNN_F32 && dtype != CRNN_BF16) return crnn_set_error(hipErrorInvalidValue, "layernorm_bwd: dtype fp32 or bf16");
-  if (M < 0 || N < 1 || lddy < N || ldx < N || (dx && lddx < N) || (dres && ldr < N))
-    return crnn_set_error(hipErrorInvalidValue, "layernorm_bwd: M >= 0, N >= 1, ld >= N");
+  if (M < 0 || N < 1 || N > kMaxN || lddy < N || ldx < N || (dx && lddx < N) || (dres && ldr < N))
+    return crnn_set_error(hipErrorInvalidValue, "layernorm_bwd: M >= 0, 1 <= N <= 2^30, ld >= N");
   if (M > 0 && (!dy || !x || !mean || !rstd)) return crnn_set_error(hipErrorInvalidValue, "layernorm_bwd: null dy / x / mean / rstd");
   if ((dw || db) && (!ws || ws_bytes < crnn_layernorm_bwd_workspace(dtype, M, N)))
     return crnn_set_error(hipErrorInvalidValue, "layernorm_bwd: workspace too small");

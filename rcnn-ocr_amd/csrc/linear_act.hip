@@ -15,20 +15,20 @@ using namespace gemm;
 namespace {
 
 // ---------------------------------------------------------------- activations
-// Phi(-|z|) = erfc(|z| / sqrt 2) / 2. For bf16 results erfc(x) = t P(t) e^{-x^2}, t = 1 / (1 + 0.435 x), P the degree-5
-// polynomial of least relative error over 0 <= x <= 9.4 (3.7e-6, fitted by reweighted least squares; half a bf16 step is
-// 3.9e-3): 15 instructions where erfcf takes several times that, and the epilogue runs them for every output.
+// Phi(-|z|) = erfc(|z| / sqrt 2) / 2 and e = exp(-z^2 / 2). For bf16 results erfc(x) = t P(t) e^{-x^2}, t = 1 / (1 + 0.435 x), P the
+// degree-5 polynomial of least relative error over 0 <= x <= 9.4 (3.7e-6, fitted by reweighted least squares; half a bf16 step
+// is 3.9e-3; the constants below carry the half and the sqrt 2): 14 instructions where erfcf takes several times that. They are
+// not hidden under the matrix instructions (one workgroup per CU): 32768 x 768 -> 1536 takes 84 us with relu, 107 with this.
 __device__ __forceinline__ float gauss_tail(float z, float& e) {
-  const float x = 0.70710678f * fabsf(z);
-  const float t = __builtin_amdgcn_rcpf(1.f + 0.435f * x);
-  e = __expf(-x * x);
-  float p = -0.15173584f;
-  p = p * t + 0.38380495f;
-  p = p * t + 0.010128383f;
-  p = p * t + 0.27484620f;
-  p = p * t + 0.23699674f;
-  p = p * t + 0.24595593f;
-  return 0.5f * p * t * e;
+  const float t = __builtin_amdgcn_rcpf(fmaf(fabsf(z), 0.30759145f, 1.f));   // 0.435 / sqrt 2
+  e = __builtin_amdgcn_exp2f(z * z * -0.72134752f);                          // log2(e) / 2
+  float p = -0.075867921f;
+  p = fmaf(p, t, 0.19190247f);
+  p = fmaf(p, t, 0.0050641913f);
+  p = fmaf(p, t, 0.13742310f);
+  p = fmaf(p, t, 0.11849837f);
+  p = fmaf(p, t, 0.12297796f);
+  return p * t * e;
 }
 template <typename T, int ACT> __device__ __forceinline__ float act(float z) {
   if constexpr (ACT == CRNN_ACT_RELU) return z > 0.f ? z : (z == z ? 0.f : z);
@@ -36,7 +36,7 @@ template <typename T, int ACT> __device__ __forceinline__ float act(float z) {
     if constexpr (sizeof(T) == 2) {
       float e;
       const float q = gauss_tail(z, e);
-      return z * (z < 0.f ? q : 1.f - q);
+      return fmaf(-fminf(fabsf(z), 20.f), q, fmaxf(z, 0.f));   // z Phi(z); the min keeps infinities off q = 0
     } else {
       return 0.5f * z * erfcf(-0.70710678118654752f * z);
     }
@@ -55,7 +55,7 @@ template <typename T> __device__ __forceinline__ float dact(int kind, float z) {
     if constexpr (sizeof(T) == 2) {
       float e;
       const float q = gauss_tail(z, e);
-      return (z < 0.f ? q : 1.f - q) + z * e * kC;
+      return fmaf(z * kC, e, 0.5f + copysignf(0.5f - q, z));
     } else {
       return 0.5f * erfcf(-0.70710678118654752f * z) + z * expf(-0.5f * z * z) * kC;
     }
@@ -183,34 +183,38 @@ int round8i(int n) { return (n + 7) & ~7; }
 bool direct(const void* p, long ld, int cols, int es) {
   return aligned16(p) && ld * es % 16 == 0 && cols % 8 == 0 && ld < 0x7fffffffL;
 }
-// rows of one launch: the loaders address an operand with 32-bit byte offsets
-long max_rows(long ld, int es) {
-  const long r = 0x7fffffffL / (ld * es);
+// rows of one launch: the loaders address an operand with 32-bit byte offsets, and a grid of 32 x 32 tiles over `cols` columns has
+// to stay under 2^32 threads
+long max_rows(long ld, int es, int cols = 1) {
+  long r = 0x7fffffffL / (ld * es);
+  const long g = (1L << 23) / ((cols + 31L) / 32) * 32;
+  if (r > g) r = g < 256 ? 256 : g;
   return r >= 256 ? r / 256 * 256 : r;
 }
 
 // columns c .. c+7 of a row of n columns at an element-aligned address, zero past its end
 typedef bf16x8 bf16x8_u __attribute__((aligned(2)));
 typedef f32x4 f32x4_u __attribute__((aligned(4)));
-template <typename T> __device__ __forceinline__ void ldrow8(const T* row, int c, int n, float* f) {
-  if (c + 8 <= n) {
+template <typename T> __device__ __forceinline__ typename VT<T>::v8 ldfrag(const T* row, int k, int K) {
+  typename VT<T>::v8 v = zero8<T>();
+  if (k + 8 <= K) {
     if constexpr (sizeof(T) == 2) {
-      const bf16x8 v = *reinterpret_cast<const bf16x8_u*>(row + c);
-      unpack8<T>(v, f);
+      v = *reinterpret_cast<const bf16x8_u*>(row + k);
     } else {
-      const f32x4 a = *reinterpret_cast<const f32x4_u*>(row + c), b = *reinterpret_cast<const f32x4_u*>(row + c + 4);
+      const f32x4 a = *reinterpret_cast<const f32x4_u*>(row + k), b = *reinterpret_cast<const f32x4_u*>(row + k + 4);
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        f[e] = a[e];
-        f[4 + e] = b[e];
+        v[e] = a[e];
+        v[4 + e] = b[e];
       }
     }
   } else {
 #pragma unroll
-    for (int e = 0; e < 8; ++e) f[e] = c + e < n ? tof(row[c + e]) : 0.f;
+    for (int e = 0; e < 8; ++e)
+      if (k + e < K) v[e] = row[k + e];
   }
+  return v;
 }
-
 // dst[rows][cols8] (zero behind cols) = src[rows][ld], up to two matrices in one launch (blockIdx.y)
 struct PadJob {
   const void* src;
@@ -225,9 +229,7 @@ template <typename T> __global__ __launch_bounds__(256) void pad_copy_kernel(Pad
   for (long i = blockIdx.x * 256L + threadIdx.x; i < n8; i += gridDim.x * 256L) {
     const long r = i / c8;
     const int c = (int)(i - r * c8) * 8;
-    float v[8];
-    ldrow8<T>((const T*)j.src + r * j.ld, c, j.cols, v);
-    st8<T>((T*)j.dst + (r * c8 + c / 8) * 8, pack8<T>(v));
+    st8<T>((T*)j.dst + (r * c8 + c / 8) * 8, ldfrag<T>((const T*)j.src + r * j.ld, c, j.cols));
   }
 }
 // copies the given jobs (src NULL: none)
@@ -270,13 +272,72 @@ int tiles_run(const LA& la, const LB& lb, const ActEpi<T, ACT>& ep, int M, int N
   }
 }
 
+// ---------------------------------------------------------------- few rows
+// M <= 16 * MT rows (single frames of running lines): the product is a read of w, so a workgroup takes 16 of its rows (output
+// columns) and its 8 waves split K: fragments straight from memory to registers (a lane holds 8 consecutive k of a row, the
+// layout of the matrix instruction's operands), no staging, and one join in LDS. Any alignment: nothing is copied first.
+// bf16 2048 x 2048 (8 MB of w), us: 4.9 / 6.2 / 8.1 at 1 / 16 / 32 rows, 10.6 in 32 x 32 tiles; 64 rows 11.6 against 10.8, so those
+// stay with the tiles (fp32: 7.9 / 10.8 / 15.5 against 19.5; 512 x 1024 bf16, launch-bound: 4.6 / 4.6 / 5.3 against 5.0).
+constexpr int SKINNY_ROWS = 32, SKW = 8;
+template <typename T, int ACT, int MT>
+__global__ __launch_bounds__(64 * SKW) void skinny_kernel(const T* __restrict__ x, long ldx, const T* __restrict__ w, long ldw,
+                                                          ActEpi<T, ACT> ep, int M, int N, int K) {
+  __shared__ f32x4 red[SKW][MT][64];
+  const int lane = threadIdx.x & 63, wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), c = lane & 15, g8 = 8 * (lane >> 4);
+  const int n0 = blockIdx.x * 16;
+  const T* wr = w + min(n0 + c, N - 1) * ldw;   // rows past the end repeat the last: their outputs are not stored
+  const T* xr[MT];
+  f32x4 acc[MT];
+#pragma unroll
+  for (int i = 0; i < MT; ++i) {
+    xr[i] = x + min(i * 16 + c, M - 1) * ldx;
+    acc[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+  }
+  constexpr int U = 4;   // steps of 32 in flight
+  for (int k0 = wid * 32; k0 < K; k0 += SKW * 32 * U) {
+    typename VT<T>::v8 b[U], a[U][MT];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int k = k0 + u * SKW * 32 + g8;
+      b[u] = ldfrag<T>(wr, k, K);
+#pragma unroll
+      for (int i = 0; i < MT; ++i) a[u][i] = ldfrag<T>(xr[i], k, K);
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+      for (int i = 0; i < MT; ++i) mma<T>(acc[i], b[u], a[u][i]);
+  }
+#pragma unroll
+  for (int i = 0; i < MT; ++i) red[wid][i][lane] = acc[i];
+  __syncthreads();
+  if (wid < MT) {
+    f32x4 v = red[0][wid][lane];
+#pragma unroll
+    for (int q = 1; q < SKW; ++q) v += red[q][wid][lane];
+    ep.store(wid * 16 + c, n0 + 4 * (lane >> 4), v, 0);
+  }
+}
+template <typename T, int ACT>
+int skinny_run(const T* x, long ldx, const T* w, long ldw, const ActEpi<T, ACT>& ep, int M, int N, int K, hipStream_t st) {
+  const dim3 grid((N + 15) / 16), block(64 * SKW);
+  if (M <= 16) hipLaunchKernelGGL((skinny_kernel<T, ACT, 1>), grid, block, 0, st, x, ldx, w, ldw, ep, M, N, K);
+  else hipLaunchKernelGGL((skinny_kernel<T, ACT, 2>), grid, block, 0, st, x, ldx, w, ldw, ep, M, N, K);
+  return (int)hipGetLastError();
+}
+
 template <typename T, int ACT>
 int fwd_act(const T* x, long ldx, const T* w, long ldw, const void* bias, int bias_f32, const T* res, long ldr, T* y, long ldy, T* z,
-            long ldz, long M, int N, int K8, hipStream_t st) {
-  const long step = max_rows(ldx, sizeof(T));
+            long ldz, long M, int N, int K, hipStream_t st) {
   const long m16 = 16 / sizeof(T);   // elements of a 16-byte vector
   const bool al = aligned16(y) && ldy % m16 == 0 && (!z || (aligned16(z) && ldz % m16 == 0)) &&
                   (!res || (aligned16(res) && ldr % m16 == 0));
+  if (M <= SKINNY_ROWS) {
+    const ActEpi<T, ACT> ep{y, z, res, bias, ldy, ldz, ldr, (int)M, N, bias_f32, al};
+    return skinny_run<T, ACT>(x, ldx, w, ldw, ep, (int)M, N, K, st);
+  }
+  const int K8 = round8i(K);   // the operands are direct: rows of whole vectors, zero behind K
+  const long step = max_rows(ldx, sizeof(T), N);
   for (long m0 = 0; m0 < M; m0 += step) {
     const int m = (int)(M - m0 < step ? M - m0 : step);
     const RowMajorK<T> la{x + m0 * ldx, (int)ldx, m, K8};
@@ -295,20 +356,21 @@ int fwd_t(const void* x, long ldx, const void* w, long ldw, const void* bias, in
   const int K8 = round8i(K);
   const T *xp = (const T*)x, *wp = (const T*)w;
   PadJob jx = {}, jw = {};
-  if (!direct(x, ldx, K, sizeof(T))) {
+  const bool few = M <= SKINNY_ROWS;
+  if (!few && !direct(x, ldx, K, sizeof(T))) {
     jx = {x, ws, ldx, M, K};
     xp = (const T*)ws;
     ldx = K8;
     ws += up256((size_t)M * K8 * sizeof(T));
   }
-  if (!direct(w, ldw, K, sizeof(T))) {
+  if (!few && !direct(w, ldw, K, sizeof(T))) {
     jw = {w, ws, ldw, N, K};
     wp = (const T*)ws;
     ldw = K8;
   }
   const int rc = pad_copy<T>(jx, jw, st);
   if (rc) return rc;
-#define FWD(A) fwd_act<T, A>(xp, ldx, wp, ldw, bias, bias_f32, (const T*)res, ldr, (T*)y, ldy, (T*)z, ldz, M, N, K8, st)
+#define FWD(A) fwd_act<T, A>(xp, ldx, wp, ldw, bias, bias_f32, (const T*)res, ldr, (T*)y, ldy, (T*)z, ldz, M, N, K, st)
   if (kind == CRNN_ACT_RELU) return FWD(CRNN_ACT_RELU);
   if (kind == CRNN_ACT_GELU) return FWD(CRNN_ACT_GELU);
   if (kind == CRNN_ACT_SILU) return FWD(CRNN_ACT_SILU);
@@ -329,18 +391,34 @@ __global__ __launch_bounds__(256) void dz_kernel(const T* __restrict__ dy, long 
   float s[8];
 #pragma unroll
   for (int e = 0; e < 8; ++e) s[e] = 0.f;
+  constexpr int R = 4;   // rows in flight
   if (n < N8)
-    for (long m = (long)blockIdx.y * 8 + rl; m < M; m += 8L * gridDim.y) {
-      float g[8], q[8];
-      ldrow8<T>(dy + m * lddy, n, N, g);
-      if (z) {
-        ldrow8<T>(z + m * ldz, n, N, q);
+    for (long mb = (long)blockIdx.y * 8 + rl; mb < M; mb += 8L * R * gridDim.y) {
+      typename VT<T>::v8 gr[R], zr[R];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) g[e] *= dact<T>(kind, q[e]);
+      for (int r = 0; r < R; ++r) {
+        const long m = mb + 8L * r * gridDim.y;
+        gr[r] = zero8<T>();
+        if (m < M) {
+          gr[r] = ldfrag<T>(dy + m * lddy, n, N);
+          if (z) zr[r] = ldfrag<T>(z + m * ldz, n, N);
+        }
       }
 #pragma unroll
-      for (int e = 0; e < 8; ++e) s[e] += g[e];
-      if (dz) st8<T>(dz + m * N8 + n, pack8<T>(g));
+      for (int r = 0; r < R; ++r) {
+        const long m = mb + 8L * r * gridDim.y;
+        if (m >= M) break;
+        float g[8], q[8];
+        unpack8<T>(gr[r], g);
+        if (z) {
+          unpack8<T>(zr[r], q);
+#pragma unroll
+          for (int e = 0; e < 8; ++e) g[e] *= dact<T>(kind, q[e]);
+        }
+#pragma unroll
+        for (int e = 0; e < 8; ++e) s[e] += g[e];
+        if (dz) st8<T>(dz + m * N8 + n, pack8<T>(g));
+      }
     }
   if (!part) return;
 #pragma unroll
@@ -418,11 +496,11 @@ __global__ __launch_bounds__(256) void reduce_kernel(const float* __restrict__ s
   }
 }
 
-// row slices of the column sums: enough workgroups for the chip, few partial rows
+// row slices of the column sums: enough workgroups for the chip (a row a lane where there are few), few partial rows to add
 int dz_slices(long M, int N) {
   const long cb = (round8i(N) + 255) / 256;
   long g = (2L * crnn_cu_count() + cb - 1) / cb;
-  const long most = (M + 31) / 32;
+  const long most = (M + 7) / 8;
   if (g > most) g = most;
   if (g > 128) g = 128;
   return (int)(g < 1 ? 1 : g);
@@ -520,7 +598,7 @@ int bwd_t(const BwdPlan& p, const void* dy, long lddy, const void* x, long ldx, 
     if ((rc = pad_copy<T>(jx, jw, st))) return rc;
   }
   if (dx && M > 0) {
-    const long step = max_rows(ldd, sizeof(T));
+    const long step = max_rows(ldd, sizeof(T), K);
     const bool al = aligned16(dx) && lddx * (long)sizeof(T) % 16 == 0;
     for (long m0 = 0; m0 < M; m0 += step) {
       const int m = (int)(M - m0 < step ? M - m0 : step);
@@ -586,7 +664,7 @@ bool too_big(int es, long ldx, long ldw, int N, int K) {
 extern "C" {
 
 size_t crnn_linear_fwd_workspace(int dtype, const void* x, long ldx, const void* w, long ldw, long M, int N, int K) {
-  if (bad_linear(dtype, 0, M, N, K)) return 0;
+  if (bad_linear(dtype, 0, M, N, K) || M <= SKINNY_ROWS) return 0;
   const int es = dtype == CRNN_BF16 ? 2 : 4;
   size_t n = 0;
   if (!direct(x, ldx, K, es)) n += up256((size_t)M * round8i(K) * es);

@@ -554,7 +554,7 @@ template <typename T, int W, bool BACK> int scan_go(const ScanArgs& a, hipStream
   constexpr int kVec = vec_of<T>();
   const int nd = a.dir == 2 ? 2 : 1;
   const long blocks = (long)a.groups * nd * a.B * a.S;
-  if (blocks > 0x7fffffffL) return crnn_set_error(hipErrorInvalidValue, "gated_scan: too many rows");
+  if (blocks > 0xffffffffL / (64 * W)) return crnn_set_error(hipErrorInvalidValue, "gated_scan: a grid of 2^32 threads or more");
   const dim3 grid((unsigned)blocks), block(64 * W);
   if (a.S > 1) {
     if constexpr (W == kWmax) {   // only the widest tiles are cut into segments

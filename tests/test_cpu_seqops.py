@@ -44,6 +44,9 @@ F3 = torch.zeros(2, 5, 6)
     lambda: crnn_hip.gated_scan(F3, F3, lengths=torch.ones(3, dtype=torch.int32)),
     lambda: crnn_hip.gated_scan(F3, F3, lengths=torch.ones(2)),
     lambda: crnn_hip.gated_scan(F3, F3, lengths=[1, 2]),
+    lambda: crnn_hip.layer_norm(torch.zeros(1).expand(1 << 31)),
+    lambda: crnn_hip.linear(torch.zeros(1).expand(1, 1 << 31), torch.zeros(1).expand(1, 1 << 31)),
+    lambda: crnn_hip.gated_scan(torch.zeros(1).expand(1, 1 << 31, 1), torch.zeros(1).expand(1, 1 << 31, 1)),
     lambda: crnn_hip.gated_scan_step(F3, F3, F3),
     lambda: crnn_hip.gated_scan_step(X, X, X[:2]),
     lambda: crnn_hip.gated_scan_step(X, X, X.bfloat16()),
@@ -93,7 +96,8 @@ def test_c_layernorm_refusals():
     bad("dtype", _0=2)
     bad("ld >= N", _2=7)
     bad("ld >= N", _6=7)
-    bad("N >= 1", _10=0)
+    bad("N <= 2", _10=0)
+    bad("N <= 2", _10=(1 << 30) + 1, _2=1 << 31, _6=1 << 31)
     bad("M >= 0", _9=-1)
     bad("go together", _7=P)
     bad("null", _1=None)
@@ -107,11 +111,12 @@ def test_c_layernorm_refusals():
 
 def test_c_linear_refusals():
     lib = L.lib()
-    assert lib.crnn_linear_fwd_workspace(1, P, 16, P, 16, 4, 8, 16) == 0                 # whole aligned vectors
-    assert lib.crnn_linear_fwd_workspace(1, P, 15, P, 15, 4, 8, 15) == 256 + 256         # both operands copied
-    assert lib.crnn_linear_fwd_workspace(1, C.c_void_p(258), 16, P, 16, 4, 8, 16) == 256  # an unaligned base
+    assert lib.crnn_linear_fwd_workspace(1, P, 16, P, 16, 99, 8, 16) == 0                # whole aligned vectors
+    assert lib.crnn_linear_fwd_workspace(1, P, 15, P, 15, 65, 8, 15) == 65 * 32 + 224 + 256  # both operands copied
+    assert lib.crnn_linear_fwd_workspace(1, P, 15, P, 15, 32, 8, 15) == 0                # few rows: read as they lie
+    assert lib.crnn_linear_fwd_workspace(1, C.c_void_p(258), 16, P, 16, 65, 8, 16) == 65 * 32 + 224  # an unaligned base
 
-    def fwd(match, dt=1, x=P, ldx=16, ldw=16, act=0, res=None, ldr=0, ldy=8, z=None, ldz=0, ws=None, n=0, M=4, N=8, K=16):
+    def fwd(match, dt=1, x=P, ldx=16, ldw=16, act=0, res=None, ldr=0, ldy=8, z=None, ldz=0, ws=None, n=0, M=99, N=8, K=16):
         _refused("crnn_linear_fwd", dt, x, ldx, P, ldw, None, 0, act, res, ldr, P, ldy, z, ldz, ws, n, M, N, K, None, match=match)
     fwd("dtype", dt=2)
     fwd("act", act=4)
