@@ -15,6 +15,7 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 PKG = os.path.dirname(HERE)
 # CRNN_HIP_LIB: an alternative build of the same library (tuning A/B runs)
 LIB_PATH = os.environ.get("CRNN_HIP_LIB", os.path.join(HERE, "libcrnn_hip.so"))
+TORCH_LIB_PATH = os.path.join(HERE, "libcrnn_torch.so")
 CSRC = os.path.join(PKG, "csrc")
 
 F32, BF16 = 0, 1
@@ -182,7 +183,7 @@ _lib = None
 
 def build(force: bool = False, jobs: int = 8) -> str:
     """Compile libcrnn_hip.so for gfx950 with hipcc (in-tree)."""
-    if force or not os.path.exists(LIB_PATH):
+    if force or not (os.path.exists(LIB_PATH) and os.path.exists(TORCH_LIB_PATH)):
         subprocess.run(["make", "-C", CSRC, f"-j{jobs}"], check=True)
     else:
         subprocess.run(["make", "-C", CSRC, f"-j{jobs}", "-q"], check=False)
@@ -264,61 +265,21 @@ def dtype_code(dt: torch.dtype) -> int:
     raise ValueError(f"unsupported compute dtype {dt}")
 
 
-_raw_stream = torch._C._cuda_getCurrentRawStream   # current_stream(i).cuda_stream without the Python Stream object (1 us)
+_ops = None
 
 
-def call_on(t: torch.Tensor, name: str, *args):
-    """call(name, *args, stream) with t's device current and that device's current torch stream"""
-    idx = t.get_device()
-    if idx == torch._C._cuda_getDevice():
-        rc = getattr(_lib or lib(), name)(*args, _raw_stream(idx))
-    else:
-        with torch.cuda.device(idx):
-            rc = getattr(_lib or lib(), name)(*args, _raw_stream(idx))
-    if rc:
-        check(rc, name)
-
-
-def rows(t: torch.Tensor):
-    """t [..., N] as M rows of N contiguous elements -> (tensor, M, row stride): t itself where its strides allow (rows one
-    constant stride >= N apart), else a contiguous copy"""
-    n = t.shape[-1]
-    if t.is_contiguous():
-        return t, t.numel() // n if n else 0, n
-    if t.dim() >= 2 and (t.stride(-1) == 1 or n == 1):
-        size, stride = t.shape[:-1], t.stride()[:-1]
-        ld = stride[-1]
-        if ld >= n and all(stride[i] == stride[i + 1] * size[i + 1] for i in range(len(size) - 1)):
-            return t, t.numel() // n, ld
-    return t.contiguous(), t.numel() // n if n else 0, n
-
-
-def check_operand(op: str, name: str, t, shape, dtype, device):
-    """ValueError unless t is a tensor of this shape (None: any), dtype (one or several) and device"""
-    if not isinstance(t, torch.Tensor):
-        raise ValueError(f"{op}: {name} must be a tensor, got {type(t).__name__}")
-    if shape is not None and tuple(t.shape) != tuple(shape):
-        raise ValueError(f"{op}: {name} must have shape {tuple(shape)}, got {tuple(t.shape)}")
-    ok = dtype if isinstance(dtype, tuple) else (dtype,)
-    if t.dtype not in ok:
-        raise ValueError(f"{op}: {name} must be {' or '.join(str(d) for d in ok)}, got {t.dtype}")
-    if t.device != device:
-        raise ValueError(f"{op}: {name} must be on {device}, got {t.device}")
-
-
-def check_sizes(op: str, *sizes):
-    """the C ABI's sizes are ints"""
-    if max(sizes) >= 1 << 31:
-        raise ValueError(f"{op}: sizes must be below 2^31, got {sizes}")
-
-
-def differentiable_once(backward):
-    """torch's once_differentiable, at its price (4 us a call) only where create_graph asks for a second derivative"""
-    guarded = torch.autograd.function.once_differentiable(backward)
-
-    def run(ctx, *grads):
-        return guarded(ctx, *grads) if torch.is_grad_enabled() else backward(ctx, *grads)
-    return run
+def ops():
+    """torch.ops.crnn, the torch binding of the sequence operators (csrc/torch_binding.cpp); loads it (once) after the library
+    whose entry points it calls. Raises if it is missing: there is no fallback."""
+    global _ops
+    if _ops is None:
+        lib()
+        if not os.path.exists(TORCH_LIB_PATH):
+            raise RuntimeError(f"libcrnn_torch.so not built ({TORCH_LIB_PATH}); run crnn_hip._lib.build() or "
+                               "`make -C rcnn-ocr_amd/csrc`")
+        torch.ops.load_library(TORCH_LIB_PATH)
+        _ops = torch.ops.crnn
+    return _ops
 
 
 def require_device(t: torch.Tensor):
