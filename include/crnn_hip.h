@@ -596,7 +596,7 @@ int crnn_linear_bwd(int dtype, const void* dy, long lddy, const void* x, long ld
 /* ------------------------------------------------------------------ gated linear recurrence
  * h_t = a_t h_{t-1} + (1 - a_t) v_t, a_t = sigmoid(f_t), per channel along the sequence; y_t = h_t. f, v, y [B][T][D] in
  * dtype, channels contiguous, batch / step strides in elements. dir 0: t = 0 .. len-1; 1: t = len-1 .. 0; 2: channels
- * [0, D/2) forward and [D/2, D) backward in time (D even; the bidirectional encoder's [forward | reverse] rows).
+ * [0, D/2) forward and [D/2, D) backward in time (D even; the bidirectional encoder's [forward | reverse] rows). T, D <= 2^30.
  * lengths (NULL: all T) int32 [B], clamped to [0, T]: steps t >= lengths[b] are not read and get y = 0.
  * h0 (NULL: 0) fp32 [B][D]: the state before the first step; hT (NULL: not stored) fp32 [B][D]: the one after the last
  * (h0 where the length is 0; hT may be h0 where the

@@ -312,7 +312,7 @@ struct GatedScanFn : public torch::autograd::Function<GatedScanFn> {
 void check_scan(const char* op, const Tensor& f, const Tensor& v, int64_t dims) {
   dtype_code(op, f);
   TORCH_CHECK_VALUE(f.dim() == dims, op, ": f must have ", dims, " axes, got ", f.sizes());
-  for (int64_t s : f.sizes()) TORCH_CHECK_VALUE(s < 1LL << 31, op, ": sizes must be below 2^31, got ", f.sizes());
+  for (int64_t s : f.sizes()) TORCH_CHECK_VALUE(s <= 1LL << 30, op, ": sizes must be at most 2^30, got ", f.sizes());
   check(op, "v", v, f.sizes(), f);
   check_type(op, "v", v, f.scalar_type(), f.scalar_type());
 }

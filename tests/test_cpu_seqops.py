@@ -77,6 +77,17 @@ def test_cpu_tensors_are_refused(call):
         call()
 
 
+def test_binding_is_required(monkeypatch):
+    """the operators are in libcrnn_torch.so, and a missing one raises instead of falling back"""
+    ops = L.ops()
+    for name in ("layer_norm", "linear", "gated_scan", "gated_scan_step"):
+        assert hasattr(ops, name)
+    monkeypatch.setattr(L, "_ops", None)
+    monkeypatch.setattr(L, "TORCH_LIB_PATH", "/nonexistent/libcrnn_torch.so")
+    with pytest.raises(RuntimeError, match="not built"):
+        L.ops()
+
+
 P = C.c_void_p(256)   # never dereferenced: every call below is refused before a launch
 
 
