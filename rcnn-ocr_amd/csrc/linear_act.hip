@@ -14,6 +14,45 @@ using namespace gemm;
 
 namespace {
 
+// ---------------------------------------------------------------- vectors at element-aligned addresses
+// (rows of any pitch: gfx950 takes unaligned vector accesses, at the price of the cache lines they straddle)
+typedef bf16x8 bf16x8_u __attribute__((aligned(2)));
+typedef bf16x4 bf16x4_u __attribute__((aligned(2)));
+typedef f32x4 f32x4_u __attribute__((aligned(4)));
+// elements k .. k+7 of a row of K, zero past its end
+template <typename T> __device__ __forceinline__ typename VT<T>::v8 ldfrag(const T* row, int k, int K) {
+  typename VT<T>::v8 v = zero8<T>();
+  if (k + 8 <= K) {
+    if constexpr (sizeof(T) == 2) {
+      v = *reinterpret_cast<const bf16x8_u*>(row + k);
+    } else {
+      const f32x4 a = *reinterpret_cast<const f32x4_u*>(row + k), b = *reinterpret_cast<const f32x4_u*>(row + k + 4);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        v[e] = a[e];
+        v[4 + e] = b[e];
+      }
+    }
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+      if (k + e < K) v[e] = row[k + e];
+  }
+  return v;
+}
+template <typename T> __device__ __forceinline__ f32x4 ld4u(const T* p) {
+  if constexpr (sizeof(T) == 4) {
+    return *reinterpret_cast<const f32x4_u*>(p);
+  } else {
+    const bf16x4 b = *reinterpret_cast<const bf16x4_u*>(p);
+    return f32x4{(float)b[0], (float)b[1], (float)b[2], (float)b[3]};
+  }
+}
+template <typename T> __device__ __forceinline__ void st4u(T* p, f32x4 v) {
+  if constexpr (sizeof(T) == 4) *reinterpret_cast<f32x4_u*>(p) = v;
+  else *reinterpret_cast<bf16x4_u*>(p) = bf16x4{(bf16)v[0], (bf16)v[1], (bf16)v[2], (bf16)v[3]};
+}
+
 // ---------------------------------------------------------------- activations
 // Phi(-|z|) = erfc(|z| / sqrt 2) / 2 and e = exp(-z^2 / 2). For bf16 results erfc(x) = t P(t) e^{-x^2}, t = 1 / (1 + 0.435 x), P the
 // degree-5 polynomial of least relative error over 0 <= x <= 9.4 (3.7e-6, fitted by reweighted least squares; half a bf16 step
@@ -76,27 +115,26 @@ template <typename T> __device__ __forceinline__ float dact(int kind, float z) {
 template <typename T, int ACT, bool OWN = false> struct ActEpi {
   static constexpr bool kStats = false;
   // the deep kernels: the wave's accumulators through its LDS, so that a lane stores 8 consecutive columns (16 bytes), and
-  // the residual's loads all in flight before the first store (one after the other, between stores that may alias them,
-  // they cost a memory latency per 64 rows x 8 columns: 139 -> see the table in DESIGN)
+  // the residual's loads all in flight before the first store (between stores that may alias them each waits for its own:
+  // 32768 x 1536 -> 768 with residual 139 us, 86 together)
   static constexpr bool kOwnTile = OWN;
   T *y, *z;
   const T* res;
   const void* bias;
   long ldy, ldz, ldr;
   int M, N, bias_f32;
-  int vec;   // y, z, res aligned for 16-byte vectors
   __device__ __forceinline__ float b(int n) const { return bias_f32 ? ((const float*)bias)[n] : tof(((const T*)bias)[n]); }
   __device__ __forceinline__ void store(int m, int n, f32x4 v, int) const {
     if (m >= M || n >= N) return;
-    if (vec && n + 4 <= N) {
-      if (bias)   // element by element: a view into a flat parameter buffer is aligned to its own type only
+    if (n + 4 <= N) {
+      if (bias)
 #pragma unroll
         for (int r = 0; r < 4; ++r) v[r] += b(n + r);
-      if (z) st4<T>(z + m * ldz + n, v);
+      if (z) st4u<T>(z + m * ldz + n, v);
 #pragma unroll
       for (int r = 0; r < 4; ++r) v[r] = act<T, ACT>(v[r]);
-      if (res) v += ld4f<T>(res + m * ldr + n);
-      st4<T>(y + m * ldy + n, v);
+      if (res) v += ld4u<T>(res + m * ldr + n);
+      st4u<T>(y + m * ldy + n, v);
       return;
     }
 #pragma unroll
@@ -119,7 +157,7 @@ template <typename T, int ACT, bool OWN = false> struct ActEpi {
     constexpr int NIT = 64 / RPI;
     const int mr = lane & 15, g = lane >> 4;
     const int c = (lane % LPR) * 8, n = cbase + c, rl = lane / LPR;
-    const bool full = vec && n + 8 <= N;  // this lane's 8 columns as vectors
+    const bool full = n + 8 <= N;         // this lane's 8 columns as vectors
     float bs[8];
 #pragma unroll
     for (int e = 0; e < 8; ++e) bs[e] = bias && n + e < N ? b(n + e) : 0.f;
@@ -130,7 +168,7 @@ template <typename T, int ACT, bool OWN = false> struct ActEpi {
 #pragma unroll
         for (int it = 0; it < NIT; ++it) {
           const int m = rbase + h * 64 + it * RPI + rl;
-          rv[it] = ld8<bf16>(res + (m < M ? m : M - 1) * ldr + n);
+          rv[it] = *reinterpret_cast<const bf16x8_u*>(res + (m < M ? m : M - 1) * ldr + n);
         }
       }
 #pragma unroll
@@ -153,14 +191,14 @@ template <typename T, int ACT, bool OWN = false> struct ActEpi {
           u[4 + e] = hi[e] + bs[4 + e];
         }
         if (m < M && full) {
-          if (z) st8<bf16>(z + m * ldz + n, pack8<bf16>(u));
+          if (z) *reinterpret_cast<bf16x8_u*>(z + m * ldz + n) = pack8<bf16>(u);
 #pragma unroll
           for (int e = 0; e < 8; ++e) u[e] = act<bf16, ACT>(u[e]);
           if (res) {
 #pragma unroll
             for (int e = 0; e < 8; ++e) u[e] += (float)rv[it][e];
           }
-          st8<bf16>(y + m * ldy + n, pack8<bf16>(u));
+          *reinterpret_cast<bf16x8_u*>(y + m * ldy + n) = pack8<bf16>(u);
         } else if (m < M) {
           for (int e = 0; e < 8 && n + e < N; ++e) {
             if (z) z[m * ldz + n + e] = (bf16)u[e];
@@ -178,8 +216,9 @@ template <typename T, int ACT, bool OWN = false> struct ActEpi {
 // ---------------------------------------------------------------- operands
 bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
 int round8i(int n) { return (n + 7) & ~7; }
-// the MFMA loaders read 16-byte vectors of 8 elements (fp32: two of 4): the base, the row pitch and the row length have to
-// be whole vectors
+// the LDS-DMA kernels and gemm.hpp's loaders read 16-byte vectors of 8 elements (fp32: two of 4): the base, the row pitch and the
+// row length have to be whole vectors. Other operands are copied into such rows for the deep kernels, and read as they lie by
+// the register-staged ones (1027 x 509 x 1021 fp32, forward / backward: 28.6 / 63.3 us with copies, 25.5 / 59.9 without).
 bool direct(const void* p, long ld, int cols, int es) {
   return aligned16(p) && ld * es % 16 == 0 && cols % 8 == 0 && ld < 0x7fffffffL;
 }
@@ -192,29 +231,6 @@ long max_rows(long ld, int es, int cols = 1) {
   return r >= 256 ? r / 256 * 256 : r;
 }
 
-// columns c .. c+7 of a row of n columns at an element-aligned address, zero past its end
-typedef bf16x8 bf16x8_u __attribute__((aligned(2)));
-typedef f32x4 f32x4_u __attribute__((aligned(4)));
-template <typename T> __device__ __forceinline__ typename VT<T>::v8 ldfrag(const T* row, int k, int K) {
-  typename VT<T>::v8 v = zero8<T>();
-  if (k + 8 <= K) {
-    if constexpr (sizeof(T) == 2) {
-      v = *reinterpret_cast<const bf16x8_u*>(row + k);
-    } else {
-      const f32x4 a = *reinterpret_cast<const f32x4_u*>(row + k), b = *reinterpret_cast<const f32x4_u*>(row + k + 4);
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        v[e] = a[e];
-        v[4 + e] = b[e];
-      }
-    }
-  } else {
-#pragma unroll
-    for (int e = 0; e < 8; ++e)
-      if (k + e < K) v[e] = row[k + e];
-  }
-  return v;
-}
 // dst[rows][cols8] (zero behind cols) = src[rows][ld], up to two matrices in one launch (blockIdx.y)
 struct PadJob {
   const void* src;
@@ -244,6 +260,36 @@ template <typename T> int pad_copy(PadJob a, PadJob b, hipStream_t st) {
   return (int)hipGetLastError();
 }
 
+// loaders of the register-staged kernels for operands as they lie (gemm.hpp's interface): element (row, k) at p[row * ld + k] ..
+template <typename T> struct RowsAny {
+  static constexpr bool kRowVec = false;
+  const T* p;
+  long ld;
+  int rows, K;
+  struct Ctx { const T* row; };
+  typedef int Prep;
+  __device__ __forceinline__ Ctx row_ctx(int r) const { return Ctx{r < rows ? p + r * ld : nullptr}; }
+  __device__ __forceinline__ Prep prep(int k0) const { return k0; }
+  __device__ __forceinline__ typename VT<T>::v8 load(const Ctx& c, Prep k0, int kofs) const {
+    return c.row ? ldfrag<T>(c.row, k0 + kofs, K) : zero8<T>();
+  }
+};
+// .. and at p[k * ld + row], 8 rows per vector
+template <typename T> struct ColsAny {
+  static constexpr bool kRowVec = true;
+  const T* p;
+  long ld;
+  int rows, K;
+  struct Ctx { int r8; };
+  typedef int Prep;
+  __device__ __forceinline__ Ctx row_ctx(int r8) const { return Ctx{r8}; }
+  __device__ __forceinline__ Prep prep(int k0) const { return k0; }
+  __device__ __forceinline__ typename VT<T>::v8 load(const Ctx& c, Prep k0, int kofs) const {
+    const int k = k0 + kofs;
+    return k < K ? ldfrag<T>(p + k * ld, c.r8, rows) : zero8<T>();
+  }
+};
+
 size_t up256(size_t n) { return (n + 255) & ~(size_t)255; }
 
 // ---------------------------------------------------------------- tile plans
@@ -254,22 +300,27 @@ size_t up256(size_t n) { return (n + 255) & ~(size_t)255; }
 // 19.8, 32 x 32 13.6), else 32 x 32 (500 x 520 x 512: 8.0 against 9.1). fp32 (exact-fp32 MFMA, 1/16 of the bf16 rate): 64 x 64
 // at four per CU or more (8192 x 1024 x 512: 84.8 us, 128 x 128 83.0, 32 x 32 101), else 32 x 32 with 64-deep stages
 // (1032 x 1024 x 512: 22.6 against 27.4 of 64 x 64; 304 x 520 x 1000: 13.1 against 28.7).
+// 0: register-staged, else the columns of the deep kernel's tile
+int deep_tile(int es, long M, int N, int K) {
+  const long cu = crnn_cu_count(), t256 = (M + 255) / 256 * ((N + 255) / 256), t128 = (M + 255) / 256 * ((N + 127) / 128);
+  if (es != 2 || K < 256 || N < 128 || t128 * 4 < cu * 3) return 0;
+  return (t256 + cu - 1) / cu * 7 <= (t128 + cu - 1) / cu * 5 ? 256 : 128;
+}
+template <typename T, int ACT, class LA, class LB>
+int staged_run(const LA& la, const LB& lb, const ActEpi<T, ACT>& ep, int M, int N, int K, hipStream_t st) {
+  const long cu = crnn_cu_count(), t64 = (long)((M + 63) / 64) * ((N + 63) / 64);
+  if (t64 >= (sizeof(T) == 2 ? cu : 4 * cu)) return launch<T, 64, 64>(la, lb, ep, M, N, K, 1, st);
+  return launch<T, 32, 32, 64>(la, lb, ep, M, N, K, 1, st);
+}
 template <typename T, int ACT, class LA, class LB>
 int tiles_run(const LA& la, const LB& lb, const ActEpi<T, ACT>& ep, int M, int N, int K, hipStream_t st) {
-  const long cu = crnn_cu_count(), t64 = (long)((M + 63) / 64) * ((N + 63) / 64);
   if constexpr (sizeof(T) == 2) {
-    const long t256 = (long)((M + 255) / 256) * ((N + 255) / 256), t128 = (long)((M + 255) / 256) * ((N + 127) / 128);
-    if (K >= 256 && N >= 128 && t128 * 4 >= cu * 3) {
-      const ActEpi<T, ACT, true> eo{ep.y, ep.z, ep.res, ep.bias, ep.ldy, ep.ldz, ep.ldr, ep.M, ep.N, ep.bias_f32, ep.vec};
-      if ((t256 + cu - 1) / cu * 7 <= (t128 + cu - 1) / cu * 5) return launch256<256, 256>(la, lb, eo, M, N, K, st);
-      return launch256<256, 128>(la, lb, eo, M, N, K, st);
-    }
-    if (t64 >= cu) return launch<T, 64, 64>(la, lb, ep, M, N, K, 1, st);
-    return launch<T, 32, 32>(la, lb, ep, M, N, K, 1, st);
-  } else {
-    if (t64 >= 4 * cu) return launch<T, 64, 64>(la, lb, ep, M, N, K, 1, st);
-    return launch<T, 32, 32, 64>(la, lb, ep, M, N, K, 1, st);
+    const int tile = deep_tile(2, M, N, K);
+    const ActEpi<T, ACT, true> eo{ep.y, ep.z, ep.res, ep.bias, ep.ldy, ep.ldz, ep.ldr, ep.M, ep.N, ep.bias_f32};
+    if (tile == 256) return launch256<256, 256>(la, lb, eo, M, N, K, st);
+    if (tile == 128) return launch256<256, 128>(la, lb, eo, M, N, K, st);
   }
+  return staged_run<T, ACT>(la, lb, ep, M, N, K, st);
 }
 
 // ---------------------------------------------------------------- few rows
@@ -329,48 +380,50 @@ int skinny_run(const T* x, long ldx, const T* w, long ldw, const ActEpi<T, ACT>&
 template <typename T, int ACT>
 int fwd_act(const T* x, long ldx, const T* w, long ldw, const void* bias, int bias_f32, const T* res, long ldr, T* y, long ldy, T* z,
             long ldz, long M, int N, int K, hipStream_t st) {
-  const long m16 = 16 / sizeof(T);   // elements of a 16-byte vector
-  const bool al = aligned16(y) && ldy % m16 == 0 && (!z || (aligned16(z) && ldz % m16 == 0)) &&
-                  (!res || (aligned16(res) && ldr % m16 == 0));
   if (M <= SKINNY_ROWS) {
-    const ActEpi<T, ACT> ep{y, z, res, bias, ldy, ldz, ldr, (int)M, N, bias_f32, al};
+    const ActEpi<T, ACT> ep{y, z, res, bias, ldy, ldz, ldr, (int)M, N, bias_f32};
     return skinny_run<T, ACT>(x, ldx, w, ldw, ep, (int)M, N, K, st);
   }
-  const int K8 = round8i(K);   // the operands are direct: rows of whole vectors, zero behind K
+  const bool any = !direct(x, ldx, K, sizeof(T)) || !direct(w, ldw, K, sizeof(T));   // then the plan is register-staged (fwd_copies)
   const long step = max_rows(ldx, sizeof(T), N);
   for (long m0 = 0; m0 < M; m0 += step) {
     const int m = (int)(M - m0 < step ? M - m0 : step);
-    const RowMajorK<T> la{x + m0 * ldx, (int)ldx, m, K8};
-    const RowMajorK<T> lb{w, (int)ldw, N, K8};
-    const ActEpi<T, ACT> ep{y + m0 * ldy, z ? z + m0 * ldz : nullptr, res ? res + m0 * ldr : nullptr, bias, ldy, ldz, ldr, m, N,
-                            bias_f32, al};
-    const int rc = tiles_run<T, ACT>(la, lb, ep, m, N, K8, st);
+    const ActEpi<T, ACT> ep{y + m0 * ldy, z ? z + m0 * ldz : nullptr, res ? res + m0 * ldr : nullptr, bias, ldy, ldz, ldr, m, N, bias_f32};
+    const int rc = any ? staged_run<T, ACT>(RowsAny<T>{x + m0 * ldx, ldx, m, K}, RowsAny<T>{w, ldw, N, K}, ep, m, N, K, st)
+                       : tiles_run<T, ACT>(RowMajorK<T>{x + m0 * ldx, (int)ldx, m, K}, RowMajorK<T>{w, (int)ldw, N, K}, ep, m, N, K, st);
     if (rc) return rc;
   }
   return 0;
 }
 
+// what the forward copies into aligned rows first: only the deep kernels ask for it
+struct FwdCopies { bool x, w; };
+FwdCopies fwd_copies(int es, const void* x, long ldx, const void* w, long ldw, long M, int N, int K) {
+  if (M <= SKINNY_ROWS || !deep_tile(es, M, N, round8i(K))) return {false, false};
+  return {!direct(x, ldx, K, es), !direct(w, ldw, K, es)};
+}
+
 template <typename T>
 int fwd_t(const void* x, long ldx, const void* w, long ldw, const void* bias, int bias_f32, int kind, const void* res, long ldr,
           void* y, long ldy, void* z, long ldz, char* ws, long M, int N, int K, hipStream_t st) {
-  const int K8 = round8i(K);
   const T *xp = (const T*)x, *wp = (const T*)w;
   PadJob jx = {}, jw = {};
-  const bool few = M <= SKINNY_ROWS;
-  if (!few && !direct(x, ldx, K, sizeof(T))) {
+  const FwdCopies cp = fwd_copies(sizeof(T), x, ldx, w, ldw, M, N, K);
+  const int K8 = round8i(K);
+  if (cp.x) {
     jx = {x, ws, ldx, M, K};
     xp = (const T*)ws;
     ldx = K8;
     ws += up256((size_t)M * K8 * sizeof(T));
   }
-  if (!few && !direct(w, ldw, K, sizeof(T))) {
+  if (cp.w) {
     jw = {w, ws, ldw, N, K};
     wp = (const T*)ws;
     ldw = K8;
   }
   const int rc = pad_copy<T>(jx, jw, st);
   if (rc) return rc;
-#define FWD(A) fwd_act<T, A>(xp, ldx, wp, ldw, bias, bias_f32, (const T*)res, ldr, (T*)y, ldy, (T*)z, ldz, M, N, K, st)
+#define FWD(A) fwd_act<T, A>(xp, ldx, wp, ldw, bias, bias_f32, (const T*)res, ldr, (T*)y, ldy, (T*)z, ldz, M, N, cp.x || cp.w ? K8 : K, st)
   if (kind == CRNN_ACT_RELU) return FWD(CRNN_ACT_RELU);
   if (kind == CRNN_ACT_GELU) return FWD(CRNN_ACT_GELU);
   if (kind == CRNN_ACT_SILU) return FWD(CRNN_ACT_SILU);
@@ -541,8 +594,9 @@ BwdPlan bwd_plan(int dtype, const void* dy, long lddy, const void* x, long ldx, 
   p.N8 = round8i(N);
   p.K8 = round8i(K);
   p.own_dz = (need_dx || need_dw) && (kind != CRNN_ACT_NONE || !direct(dy, lddy, N, es));
-  p.copy_x = need_dw && !direct(x, ldx, K, es);
-  p.copy_w = need_dx && !direct(w, ldw, K, es);
+  // the products' other operands: copied for the deep kernels only
+  p.copy_x = need_dw && !direct(x, ldx, K, es) && dw_plan(es, p.N8, p.K8, M).tile == 256;
+  p.copy_w = need_dx && !direct(w, ldw, K, es) && deep_tile(es, M, K, p.N8);
   p.slices = need_db ? dz_slices(M, N) : 0;
   const long ldz_ = p.own_dz ? p.N8 : lddy, ldx_ = p.copy_x ? p.K8 : ldx;
   if (need_dw && M > 0) {
@@ -599,13 +653,16 @@ int bwd_t(const BwdPlan& p, const void* dy, long lddy, const void* x, long ldx, 
   }
   if (dx && M > 0) {
     const long step = max_rows(ldd, sizeof(T), K);
-    const bool al = aligned16(dx) && lddx * (long)sizeof(T) % 16 == 0;
     for (long m0 = 0; m0 < M; m0 += step) {
       const int m = (int)(M - m0 < step ? M - m0 : step);
       const RowMajorK<T> la{dzp + m0 * ldd, (int)ldd, m, p.N8};
-      const ColMajorK<T> lb{wp, (int)ldw, p.K8, N};
-      const ActEpi<T, CRNN_ACT_NONE> ep{(T*)dx + m0 * lddx, nullptr, nullptr, nullptr, lddx, 0, 0, m, K, 0, al};
-      if ((rc = tiles_run<T, CRNN_ACT_NONE>(la, lb, ep, m, K, p.N8, st))) return rc;
+      const ActEpi<T, CRNN_ACT_NONE> ep{(T*)dx + m0 * lddx, nullptr, nullptr, nullptr, lddx, 0, 0, m, K, 0};
+      // (columns behind K of a copied w are zero and not stored)
+      if (direct(wp, ldw, p.copy_w ? p.K8 : K, sizeof(T)))
+        rc = tiles_run<T, CRNN_ACT_NONE>(la, ColMajorK<T>{wp, (int)ldw, p.K8, N}, ep, m, K, p.N8, st);
+      else
+        rc = staged_run<T, CRNN_ACT_NONE>(la, ColsAny<T>{wp, ldw, K, N}, ep, m, K, p.N8, st);
+      if (rc) return rc;
     }
   }
   const float* slab = (const float*)(ws + p.o_slab);
@@ -616,14 +673,17 @@ int bwd_t(const BwdPlan& p, const void* dy, long lddy, const void* x, long ldx, 
       const int m = (int)(M - m0 < step ? M - m0 : step);
       const DwPlan d = dw_plan(sizeof(T), p.N8, p.K8, m);
       const ColMajorK<T> la{dzp + m0 * ldd, (int)ldd, p.N8, m};
-      const ColMajorK<T> lb{xp + m0 * ldx, (int)ldx, p.K8, m};
       const SlabEpi ep{(float*)(ws + p.o_slab) + (size_t)S * p.N8 * p.K8, p.N8, p.K8};
-      if constexpr (sizeof(T) == 2) {
-        if (d.tile == 256) rc = launch256<256, 256>(la, lb, ep, p.N8, p.K8, m, st, d.splits);
-        else if (d.tile == 128) rc = launch<T, 128, 128>(la, lb, ep, p.N8, p.K8, m, d.splits, st);
-        else rc = launch<T, 64, 64>(la, lb, ep, p.N8, p.K8, m, d.splits, st);
+      auto staged = [&](auto lb) {
+        return sizeof(T) == 2 && d.tile != 64 ? launch<T, 128, 128>(la, lb, ep, p.N8, p.K8, m, d.splits, st)
+                                              : launch<T, 64, 64>(la, lb, ep, p.N8, p.K8, m, d.splits, st);
+      };
+      if (direct(xp, ldx, p.copy_x ? p.K8 : K, sizeof(T))) {
+        const ColMajorK<T> lb{xp + m0 * ldx, (int)ldx, p.K8, m};
+        if constexpr (sizeof(T) == 2) rc = d.tile == 256 ? launch256<256, 256>(la, lb, ep, p.N8, p.K8, m, st, d.splits) : staged(lb);
+        else rc = staged(lb);
       } else {
-        rc = launch<T, 64, 64>(la, lb, ep, p.N8, p.K8, m, d.splits, st);
+        rc = staged(ColsAny<T>{xp + m0 * ldx, ldx, K, m});   // (its columns behind K are zero)
       }
       if (rc) return rc;
       S += d.splits;
@@ -664,12 +724,10 @@ bool too_big(int es, long ldx, long ldw, int N, int K) {
 extern "C" {
 
 size_t crnn_linear_fwd_workspace(int dtype, const void* x, long ldx, const void* w, long ldw, long M, int N, int K) {
-  if (bad_linear(dtype, 0, M, N, K) || M <= SKINNY_ROWS) return 0;
+  if (bad_linear(dtype, 0, M, N, K)) return 0;
   const int es = dtype == CRNN_BF16 ? 2 : 4;
-  size_t n = 0;
-  if (!direct(x, ldx, K, es)) n += up256((size_t)M * round8i(K) * es);
-  if (!direct(w, ldw, K, es)) n += up256((size_t)N * round8i(K) * es);
-  return n;
+  const FwdCopies cp = fwd_copies(es, x, ldx, w, ldw, M, N, K);
+  return (cp.x ? up256((size_t)M * round8i(K) * es) : 0) + (cp.w ? up256((size_t)N * round8i(K) * es) : 0);
 }
 
 int crnn_linear_fwd(int dtype, const void* x, long ldx, const void* w, long ldw, const void* bias, int bias_f32, int act, const void* res,

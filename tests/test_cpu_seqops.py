@@ -122,10 +122,15 @@ def test_c_layernorm_refusals():
 
 def test_c_linear_refusals():
     lib = L.lib()
-    assert lib.crnn_linear_fwd_workspace(1, P, 16, P, 16, 99, 8, 16) == 0                # whole aligned vectors
-    assert lib.crnn_linear_fwd_workspace(1, P, 15, P, 15, 65, 8, 15) == 65 * 32 + 224 + 256  # both operands copied
-    assert lib.crnn_linear_fwd_workspace(1, P, 15, P, 15, 32, 8, 15) == 0                # few rows: read as they lie
-    assert lib.crnn_linear_fwd_workspace(1, C.c_void_p(258), 16, P, 16, 65, 8, 16) == 65 * 32 + 224  # an unaligned base
+    # the deep kernels (256 rows a tile, three quarters of the CUs or more) take whole aligned vectors only: others are copied
+    up = lambda n: (n + 255) // 256 * 256  # noqa: E731
+    assert lib.crnn_linear_fwd_workspace(1, P, 264, P, 264, 25600, 256, 264) == 0
+    assert lib.crnn_linear_fwd_workspace(1, P, 257, P, 257, 25600, 256, 257) == up(25600 * 264 * 2) + up(256 * 264 * 2)
+    assert lib.crnn_linear_fwd_workspace(1, C.c_void_p(258), 264, P, 264, 25600, 256, 264) == up(25600 * 264 * 2)
+    # the register-staged ones, fp32 and the few-row kernel read them as they lie
+    assert lib.crnn_linear_fwd_workspace(1, P, 257, P, 257, 1000, 256, 257) == 0
+    assert lib.crnn_linear_fwd_workspace(0, P, 257, P, 257, 25600, 256, 257) == 0
+    assert lib.crnn_linear_fwd_workspace(1, P, 257, P, 257, 32, 256, 257) == 0
 
     def fwd(match, dt=1, x=P, ldx=16, ldw=16, act=0, res=None, ldr=0, ldy=8, z=None, ldz=0, ws=None, n=0, M=99, N=8, K=16):
         _refused("crnn_linear_fwd", dt, x, ldx, P, ldw, None, 0, act, res, ldr, P, ldy, z, ldz, ws, n, M, N, K, None, match=match)
@@ -140,8 +145,9 @@ def test_c_linear_refusals():
     fwd("row stride", z=P, ldz=7)
     fwd("row stride", res=P, ldr=7)
     fwd("null", x=None)
-    fwd("workspace", ldx=17, ws=P, n=1)
-    fwd("workspace", ldx=17)
+    big = dict(M=25600, N=256, K=264, ldx=265, ldw=264, ldy=256)
+    fwd("workspace", ws=P, n=1, **big)
+    fwd("workspace", **big)
     fwd("2 GiB", ldw=1 << 28)
     assert lib.crnn_linear_fwd(1, None, 16, None, 16, None, 0, 0, None, 0, None, 8, None, 0, None, 0, 0, 8, 16, None) == 0
 
