@@ -18,46 +18,12 @@ namespace {
 typedef bf16x8 bf16x8_u __attribute__((aligned(2)));
 typedef f32x4 f32x4_u __attribute__((aligned(4)));
 
-template <typename T> __device__ __forceinline__ void ldu8(const T* p, float* f) {
-  if constexpr (sizeof(T) == 2) {
-    const bf16x8 v = *reinterpret_cast<const bf16x8_u*>(p);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) f[i] = (float)v[i];
-  } else {
-    const f32x4 a = *reinterpret_cast<const f32x4_u*>(p), b = *reinterpret_cast<const f32x4_u*>(p + 4);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      f[i] = a[i];
-      f[4 + i] = b[i];
-    }
-  }
-}
-template <typename T> __device__ __forceinline__ void stu8(T* p, const float* f) {
-  if constexpr (sizeof(T) == 2) {
-    *reinterpret_cast<bf16x8_u*>(p) = pack8<bf16>(f);
-  } else {
-    f32x4 a, b;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      a[i] = f[i];
-      b[i] = f[4 + i];
-    }
-    *reinterpret_cast<f32x4_u*>(p) = a;
-    *reinterpret_cast<f32x4_u*>(p + 4) = b;
-  }
-}
-// columns c .. c+7 of a row of n columns, `fill` past its end
-template <typename T> __device__ __forceinline__ void ldrow8(const T* row, int c, int n, float* f, float fill) {
-  if (c + 8 <= n) {
-    ldu8<T>(row + c, f);
-  } else {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) f[i] = c + i < n ? tof(row[c + i]) : fill;
-  }
-}
-// the same, still packed (a row in flight)
+// columns c .. c+7 of a row of n columns, `fill` past its end (at most one lane of a row has a part of its 8 columns: for the
+// others the element-wise branch is skipped whole)
 template <typename T> __device__ __forceinline__ typename VT<T>::v8 ldraw8(const T* row, int c, int n, float fill) {
   typename VT<T>::v8 v;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) v[i] = fromf<T>(fill);
   if (c + 8 <= n) {
     if constexpr (sizeof(T) == 2) {
       v = *reinterpret_cast<const bf16x8_u*>(row + c);
@@ -69,18 +35,27 @@ template <typename T> __device__ __forceinline__ typename VT<T>::v8 ldraw8(const
         v[4 + i] = b[i];
       }
     }
-  } else {
+  } else if (c < n) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = c + i < n ? row[c + i] : fromf<T>(fill);
+    for (int i = 0; i < 7; ++i)
+      if (c + i < n) v[i] = row[c + i];
   }
   return v;
 }
+template <typename T> __device__ __forceinline__ void ldrow8(const T* row, int c, int n, float* f, float fill) {
+  unpack8<T>(ldraw8<T>(row, c, n, fill), f);
+}
 template <typename T> __device__ __forceinline__ void strow8(T* row, int c, int n, const float* f) {
   if (c + 8 <= n) {
-    stu8<T>(row + c, f);
-  } else {
+    if constexpr (sizeof(T) == 2) {
+      *reinterpret_cast<bf16x8_u*>(row + c) = pack8<bf16>(f);
+    } else {
+      *reinterpret_cast<f32x4_u*>(row + c) = f32x4{f[0], f[1], f[2], f[3]};
+      *reinterpret_cast<f32x4_u*>(row + c + 4) = f32x4{f[4], f[5], f[6], f[7]};
+    }
+  } else if (c < n) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i)
+    for (int i = 0; i < 7; ++i)
       if (c + i < n) row[c + i] = fromf<T>(f[i]);
   }
 }

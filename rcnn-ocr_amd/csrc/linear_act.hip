@@ -33,9 +33,9 @@ template <typename T> __device__ __forceinline__ typename VT<T>::v8 ldfrag(const
         v[4 + e] = b[e];
       }
     }
-  } else {
+  } else if (k < K) {
 #pragma unroll
-    for (int e = 0; e < 8; ++e)
+    for (int e = 0; e < 7; ++e)
       if (k + e < K) v[e] = row[k + e];
   }
   return v;
@@ -593,10 +593,11 @@ BwdPlan bwd_plan(int dtype, const void* dy, long lddy, const void* x, long ldx, 
   BwdPlan p = {};
   p.N8 = round8i(N);
   p.K8 = round8i(K);
-  p.own_dz = (need_dx || need_dw) && (kind != CRNN_ACT_NONE || !direct(dy, lddy, N, es));
-  // the products' other operands: copied for the deep kernels only
-  p.copy_x = need_dw && !direct(x, ldx, K, es) && dw_plan(es, p.N8, p.K8, M).tile == 256;
-  p.copy_w = need_dx && !direct(w, ldw, K, es) && deep_tile(es, M, K, p.N8);
+  // operands that are not whole aligned vectors are copied for the deep kernels only; without an activation dy is dz
+  const bool deep_dx = need_dx && deep_tile(es, M, K, p.N8), deep_dw = need_dw && dw_plan(es, p.N8, p.K8, M).tile == 256;
+  p.own_dz = (need_dx || need_dw) && (kind != CRNN_ACT_NONE || (!direct(dy, lddy, N, es) && (deep_dx || deep_dw)));
+  p.copy_x = !direct(x, ldx, K, es) && deep_dw;
+  p.copy_w = !direct(w, ldw, K, es) && deep_dx;
   p.slices = need_db ? dz_slices(M, N) : 0;
   const long ldz_ = p.own_dz ? p.N8 : lddy, ldx_ = p.copy_x ? p.K8 : ldx;
   if (need_dw && M > 0) {
@@ -637,6 +638,7 @@ int bwd_t(const BwdPlan& p, const void* dy, long lddy, const void* x, long ldx, 
       ldd = p.N8;
     }
   }
+  const bool dz_direct = p.own_dz || direct(dy, lddy, N, sizeof(T));
   if (M > 0) {
     PadJob jx = {}, jw = {};
     if (p.copy_x) {
@@ -655,13 +657,13 @@ int bwd_t(const BwdPlan& p, const void* dy, long lddy, const void* x, long ldx, 
     const long step = max_rows(ldd, sizeof(T), K);
     for (long m0 = 0; m0 < M; m0 += step) {
       const int m = (int)(M - m0 < step ? M - m0 : step);
-      const RowMajorK<T> la{dzp + m0 * ldd, (int)ldd, m, p.N8};
       const ActEpi<T, CRNN_ACT_NONE> ep{(T*)dx + m0 * lddx, nullptr, nullptr, nullptr, lddx, 0, 0, m, K, 0};
-      // (columns behind K of a copied w are zero and not stored)
-      if (direct(wp, ldw, p.copy_w ? p.K8 : K, sizeof(T)))
-        rc = tiles_run<T, CRNN_ACT_NONE>(la, ColMajorK<T>{wp, (int)ldw, p.K8, N}, ep, m, K, p.N8, st);
+      // (columns behind K of a copied w, and behind N of an own dz, are zero)
+      if (dz_direct && direct(wp, ldw, p.copy_w ? p.K8 : K, sizeof(T)))
+        rc = tiles_run<T, CRNN_ACT_NONE>(RowMajorK<T>{dzp + m0 * ldd, (int)ldd, m, p.N8}, ColMajorK<T>{wp, (int)ldw, p.K8, N}, ep, m, K,
+                                         p.N8, st);
       else
-        rc = staged_run<T, CRNN_ACT_NONE>(la, ColsAny<T>{wp, ldw, K, N}, ep, m, K, p.N8, st);
+        rc = staged_run<T, CRNN_ACT_NONE>(RowsAny<T>{dzp + m0 * ldd, ldd, m, N}, ColsAny<T>{wp, ldw, K, N}, ep, m, K, p.N8, st);
       if (rc) return rc;
     }
   }
@@ -672,18 +674,17 @@ int bwd_t(const BwdPlan& p, const void* dy, long lddy, const void* x, long ldx, 
     for (long m0 = 0; m0 < M; m0 += step) {
       const int m = (int)(M - m0 < step ? M - m0 : step);
       const DwPlan d = dw_plan(sizeof(T), p.N8, p.K8, m);
-      const ColMajorK<T> la{dzp + m0 * ldd, (int)ldd, p.N8, m};
       const SlabEpi ep{(float*)(ws + p.o_slab) + (size_t)S * p.N8 * p.K8, p.N8, p.K8};
-      auto staged = [&](auto lb) {
+      auto staged = [&](auto la, auto lb) {
         return sizeof(T) == 2 && d.tile != 64 ? launch<T, 128, 128>(la, lb, ep, p.N8, p.K8, m, d.splits, st)
                                               : launch<T, 64, 64>(la, lb, ep, p.N8, p.K8, m, d.splits, st);
       };
-      if (direct(xp, ldx, p.copy_x ? p.K8 : K, sizeof(T))) {
-        const ColMajorK<T> lb{xp + m0 * ldx, (int)ldx, p.K8, m};
-        if constexpr (sizeof(T) == 2) rc = d.tile == 256 ? launch256<256, 256>(la, lb, ep, p.N8, p.K8, m, st, d.splits) : staged(lb);
-        else rc = staged(lb);
-      } else {
-        rc = staged(ColsAny<T>{xp + m0 * ldx, ldx, K, m});   // (its columns behind K are zero)
+      if (dz_direct && direct(xp, ldx, p.copy_x ? p.K8 : K, sizeof(T))) {
+        const ColMajorK<T> la{dzp + m0 * ldd, (int)ldd, p.N8, m}, lb{xp + m0 * ldx, (int)ldx, p.K8, m};
+        if constexpr (sizeof(T) == 2) rc = d.tile == 256 ? launch256<256, 256>(la, lb, ep, p.N8, p.K8, m, st, d.splits) : staged(la, lb);
+        else rc = staged(la, lb);
+      } else {   // (rows of dz behind N and columns of x behind K are zero)
+        rc = staged(ColsAny<T>{dzp + m0 * ldd, ldd, N, m}, ColsAny<T>{xp + m0 * ldx, ldx, K, m});
       }
       if (rc) return rc;
       S += d.splits;

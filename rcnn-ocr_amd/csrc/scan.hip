@@ -539,8 +539,10 @@ Plan scan_plan(int dtype, int B, int T, int D, int dir) {
   while (p.W < wmax && T > p.W * L) p.W *= 2;
   p.tiles = (T + p.W * L - 1) / (p.W * L);   // T <= kMaxT: no overflow
   p.S = 1;
-  // two workgroups per CU (2 x 16384 x 1024 bf16, forward / backward: 57 / 89 us; 58 / 95 at three, 61 / 97 at four)
-  if (p.W == kWmax && rows < cu && p.tiles > 2) {
+  // Segments where rows leave half of the CUs idle, or some of them for long (forward / backward, us, with segments and without:
+  // 96 rows of 300 steps 12.8 / 16.0, 13.4 / 20.3; 200 of 300 19.0 / 24.1, 14.7 / 22.5; 160 of 512 22 / 30, 20 / 33; 192 of 2000
+  // 85 / 146, 85 / 163). Two workgroups per CU (2 x 16384 x 1024 bf16: 57 / 89; 58 / 95 at three, 61 / 97 at four).
+  if (p.W == kWmax && p.tiles > 2 && (2 * rows < cu || (rows < cu && p.tiles > 24))) {
     long s = (2 * cu + rows - 1) / rows;
     if (s > p.tiles / 2) s = p.tiles / 2;
     if (s > 128) s = 128;
