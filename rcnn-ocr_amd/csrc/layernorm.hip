@@ -6,9 +6,11 @@
 //
 // Both passes are bound by memory: the forward reads x and writes y, the backward reads x, dy and writes dx. A row lives
 // in registers (8 consecutive elements per lane and chunk), so each is read once: WPR waves own a row of up to
-// WPR * 64 * 8 * KC columns. Rows wider than the widest such tile loop over memory (the *_wide kernels).
+// WPR * 64 * 8 * KC columns, and narrow rows share a wave, LPR lanes each. Rows wider than the widest such tile loop over
+// memory (the *_wide kernels).
 // The weight gradients sum over rows: a wave keeps its columns' sums in registers over all the rows it walks, the
 // workgroup joins its waves in LDS and writes one partial row, and ln_colsum adds the partial rows in a fixed order.
+#include <type_traits>
 #include "common.hpp"
 #include "crnn_internal.hpp"
 
@@ -60,19 +62,24 @@ template <typename T> __device__ __forceinline__ void strow8(T* row, int c, int 
   }
 }
 
-// sum of a and of b over the 64 lanes (every lane gets both)
-__device__ __forceinline__ void wave_sum2(float& a, float& b) {
-  a = rowgroup_sum<16>(a);
-  b = rowgroup_sum<16>(b);
-  a += __shfl_xor(a, 16, 64);
-  b += __shfl_xor(b, 16, 64);
-  a += __shfl_xor(a, 32, 64);
-  b += __shfl_xor(b, 32, 64);
+// sum of a and of b over aligned groups of LPR lanes (every lane gets both)
+template <int LPR = 64> __device__ __forceinline__ void wave_sum2(float& a, float& b) {
+  a = rowgroup_sum<LPR < 16 ? LPR : 16>(a);
+  b = rowgroup_sum<LPR < 16 ? LPR : 16>(b);
+  if constexpr (LPR >= 32) {
+    a += __shfl_xor(a, 16, 64);
+    b += __shfl_xor(b, 16, 64);
+  }
+  if constexpr (LPR >= 64) {
+    a += __shfl_xor(a, 32, 64);
+    b += __shfl_xor(b, 32, 64);
+  }
 }
 // ... over the WPR waves of a row; red: 2 * WPR floats of LDS, two sets used in turn (`set`), so that one barrier per sum is
 // enough
-template <int WPR> __device__ __forceinline__ void row_sum2(float& a, float& b, float (*red)[2 * WPR], int set, int wid) {
-  wave_sum2(a, b);
+template <int WPR, int LPR> __device__ __forceinline__ void row_sum2(float& a, float& b, float (*red)[2 * WPR], int set, int wid) {
+  static_assert(WPR == 1 || LPR == 64, "whole waves");
+  wave_sum2<LPR>(a, b);
   if constexpr (WPR > 1) {
     if ((threadIdx.x & 63) == 0) {
       red[set][2 * wid] = a;
@@ -90,7 +97,7 @@ template <int WPR> __device__ __forceinline__ void row_sum2(float& a, float& b, 
 
 // mean and rstd of the row in x (KC chunks of 8 per lane): the plain mean first, then the deviations from it, whose own
 // sum corrects the mean's rounding (a row far off centre keeps its variance)
-template <int WPR, int KC>
+template <int WPR, int KC, int LPR>
 __device__ __forceinline__ void row_stats(const float (*x)[8], const int* c, int N, float eps, float (*red)[2 * WPR],
                                           int wid, float& mean, float& rstd) {
   const float inv = 1.f / (float)N;
@@ -99,7 +106,7 @@ __device__ __forceinline__ void row_stats(const float (*x)[8], const int* c, int
   for (int k = 0; k < KC; ++k)
 #pragma unroll
     for (int i = 0; i < 8; ++i) s += x[k][i];   // 0 past the end
-  row_sum2<WPR>(s, z, red, 0, wid);
+  row_sum2<WPR, LPR>(s, z, red, 0, wid);
   const float m0 = s * inv;
   float d = 0.f, q = 0.f;
 #pragma unroll
@@ -110,17 +117,17 @@ __device__ __forceinline__ void row_stats(const float (*x)[8], const int* c, int
       d += e;
       q += e * e;
     }
-  row_sum2<WPR>(d, q, red, 1, wid);
+  row_sum2<WPR, LPR>(d, q, red, 1, wid);
   d *= inv;
   mean = m0 + d;
   rstd = 1.f / sqrtf(fmaxf(q * inv - d * d, 0.f) + eps);
 }
 
-// rows per workgroup pass: 4 waves, one row each (WPR = 1), or one row on all WPR waves
+// rows per workgroup pass: 4 waves of 64 / LPR rows (WPR = 1), or one row on all WPR waves
 template <int WPR> constexpr int ln_threads() { return WPR == 1 ? 256 : WPR * 64; }
-template <int WPR> constexpr int ln_rpb() { return WPR == 1 ? 4 : 1; }
+template <int WPR, int LPR> constexpr int ln_rpb() { return WPR == 1 ? 4 * (64 / LPR) : 1; }
 
-template <typename T, int WPR, int KC>
+template <typename T, int WPR, int KC, int LPR>
 __global__ __launch_bounds__(ln_threads<WPR>()) void ln_fwd_kernel(const T* __restrict__ x, long ldx, const float* __restrict__ w,
                                                                    const float* __restrict__ b, T* __restrict__ y, long ldy,
                                                                    float* __restrict__ mean, float* __restrict__ rstd, long M,
@@ -128,11 +135,12 @@ __global__ __launch_bounds__(ln_threads<WPR>()) void ln_fwd_kernel(const T* __re
   __shared__ float red[2][2 * WPR];
   const int lane = threadIdx.x & 63, wid = threadIdx.x >> 6;
   const int wr = WPR == 1 ? 0 : wid;
+  const int lr = lane % LPR, sub = lane / LPR;   // lane of its row, row of the wave
   int c[KC];
   float wv[KC][8], bv[KC][8];
 #pragma unroll
   for (int k = 0; k < KC; ++k) {
-    c[k] = ((k * WPR + wr) * 64 + lane) * 8;
+    c[k] = ((k * WPR + wr) * LPR + lr) * 8;
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       wv[k][i] = 1.f;
@@ -141,13 +149,16 @@ __global__ __launch_bounds__(ln_threads<WPR>()) void ln_fwd_kernel(const T* __re
     if (w) ldrow8<float>(w, c[k], N, wv[k], 0.f);
     if (b) ldrow8<float>(b, c[k], N, bv[k], 0.f);
   }
-  for (long m = (long)blockIdx.x * ln_rpb<WPR>() + (WPR == 1 ? wid : 0); m < M; m += (long)gridDim.x * ln_rpb<WPR>()) {
+  constexpr long RPB = ln_rpb<WPR, LPR>();
+  for (long mb = (long)blockIdx.x * RPB + (WPR == 1 ? wid * (64 / LPR) : 0); mb < M; mb += (long)gridDim.x * RPB) {
+    const long m = mb + sub;
+    const int n = LPR == 64 || m < M ? N : 0;   // columns of this lane's row: none past the last one
     float v[KC][8];
 #pragma unroll
-    for (int k = 0; k < KC; ++k) ldrow8<T>(x + m * ldx, c[k], N, v[k], 0.f);
+    for (int k = 0; k < KC; ++k) ldrow8<T>(x + m * ldx, c[k], n, v[k], 0.f);
     float mu, rs;
-    row_stats<WPR, KC>(v, c, N, eps, red, wr, mu, rs);
-    if (mean && lane == 0 && wr == 0) {
+    row_stats<WPR, KC, LPR>(v, c, N, eps, red, wr, mu, rs);
+    if (mean && lr == 0 && wr == 0 && (LPR == 64 || n)) {
       mean[m] = mu;
       rstd[m] = rs;
     }
@@ -155,29 +166,30 @@ __global__ __launch_bounds__(ln_threads<WPR>()) void ln_fwd_kernel(const T* __re
     for (int k = 0; k < KC; ++k) {
 #pragma unroll
       for (int i = 0; i < 8; ++i) v[k][i] = (v[k][i] - mu) * rs * wv[k][i] + bv[k][i];
-      strow8<T>(y + m * ldy, c[k], N, v[k]);
+      strow8<T>(y + m * ldy, c[k], n, v[k]);
     }
   }
 }
 
-template <typename T, int WPR, int KC>
+template <typename T, int WPR, int KC, int LPR>
 __global__ __launch_bounds__(ln_threads<WPR>(), WPR == 1 ? 3 : 1) void ln_bwd_kernel(const T* __restrict__ dy, long lddy, const T* __restrict__ x,
                                                                    long ldx, const float* __restrict__ w,
                                                                    const float* __restrict__ mean, const float* __restrict__ rstd,
                                                                    const T* dres, long ldr, T* dx, long lddx,
                                                                    float* __restrict__ part, long M, int N) {
-  constexpr int NW = ln_threads<WPR>() / 64;
-  constexpr int COLS = WPR * KC * 512;
+  constexpr int NV = ln_threads<WPR>() / LPR;   // row lanes of the workgroup
+  constexpr int COLS = WPR * KC * LPR * 8;
   __shared__ float red[2][2 * WPR];
-  __shared__ __attribute__((aligned(16))) float join[WPR == 1 ? NW * COLS : 4];
+  __shared__ __attribute__((aligned(16))) float join[WPR == 1 ? NV * COLS : 4];
   const int lane = threadIdx.x & 63, wid = threadIdx.x >> 6;
   const int wr = WPR == 1 ? 0 : wid;
   const float inv = 1.f / (float)N;
+  const int lr = lane % LPR, sub = lane / LPR;
   int c[KC];
   float wv[KC][8], sw[KC][8], sb[KC][8];
 #pragma unroll
   for (int k = 0; k < KC; ++k) {
-    c[k] = ((k * WPR + wr) * 64 + lane) * 8;
+    c[k] = ((k * WPR + wr) * LPR + lr) * 8;
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       wv[k][i] = 1.f;
@@ -186,29 +198,31 @@ __global__ __launch_bounds__(ln_threads<WPR>(), WPR == 1 ? 3 : 1) void ln_bwd_ke
     if (w) ldrow8<float>(w, c[k], N, wv[k], 0.f);
   }
   int set = 0;
-  const long step = (long)gridDim.x * ln_rpb<WPR>();
-  long m = (long)blockIdx.x * ln_rpb<WPR>() + (WPR == 1 ? wid : 0);
+  constexpr long RPB = ln_rpb<WPR, LPR>();
+  const long step = (long)gridDim.x * RPB;
+  long mb = (long)blockIdx.x * RPB + (WPR == 1 ? wid * (64 / LPR) : 0);
   typename VT<T>::v8 xr[KC], gr[KC];   // the next row, on its way while this one is worked on
-  if (m < M)
+  auto fetch = [&](long m) {
+    const int n = LPR == 64 || m < M ? N : 0;
 #pragma unroll
     for (int k = 0; k < KC; ++k) {
-      xr[k] = ldraw8<T>(x + m * ldx, c[k], N, 0.f);
-      gr[k] = ldraw8<T>(dy + m * lddy, c[k], N, 0.f);
+      xr[k] = ldraw8<T>(x + m * ldx, c[k], n, 0.f);
+      gr[k] = ldraw8<T>(dy + m * lddy, c[k], n, 0.f);
     }
-  for (; m < M; m += step) {
-    const float mu = mean[m], rs = rstd[m];
+  };
+  if (mb < M) fetch(mb + sub);
+  for (; mb < M; mb += step) {
+    const long m = mb + sub;
+    const int n = LPR == 64 || m < M ? N : 0;   // columns of this lane's row: none past the last one
+    const bool live = LPR == 64 || n;
+    const float mu = live ? mean[m] : 0.f, rs = live ? rstd[m] : 0.f;
     float xh[KC][8], g[KC][8];
 #pragma unroll
     for (int k = 0; k < KC; ++k) {
       unpack8<T>(xr[k], xh[k]);
       unpack8<T>(gr[k], g[k]);
     }
-    if (m + step < M)
-#pragma unroll
-      for (int k = 0; k < KC; ++k) {
-        xr[k] = ldraw8<T>(x + (m + step) * ldx, c[k], N, 0.f);
-        gr[k] = ldraw8<T>(dy + (m + step) * lddy, c[k], N, 0.f);
-      }
+    if (mb + step < M) fetch(m + step);
     float s1 = 0.f, s2 = 0.f;
 #pragma unroll
     for (int k = 0; k < KC; ++k)
@@ -221,7 +235,7 @@ __global__ __launch_bounds__(ln_threads<WPR>(), WPR == 1 ? 3 : 1) void ln_bwd_ke
         s1 += g[k][i];
         s2 += g[k][i] * xh[k][i];
       }
-    row_sum2<WPR>(s1, s2, red, set, wr);
+    row_sum2<WPR, LPR>(s1, s2, red, set, wr);
     set ^= 1;
     s1 *= inv;
     s2 *= inv;
@@ -232,11 +246,11 @@ __global__ __launch_bounds__(ln_threads<WPR>(), WPR == 1 ? 3 : 1) void ln_bwd_ke
         for (int i = 0; i < 8; ++i) g[k][i] = rs * (g[k][i] - s1 - xh[k][i] * s2);
         if (dres) {
           float r[8];
-          ldrow8<T>(dres + m * ldr, c[k], N, r, 0.f);
+          ldrow8<T>(dres + m * ldr, c[k], n, r, 0.f);
 #pragma unroll
           for (int i = 0; i < 8; ++i) g[k][i] += r[i];
         }
-        strow8<T>(dx + m * lddx, c[k], N, g[k]);
+        strow8<T>(dx + m * lddx, c[k], n, g[k]);
       }
     }
   }
@@ -257,13 +271,14 @@ __global__ __launch_bounds__(ln_threads<WPR>(), WPR == 1 ? 3 : 1) void ln_bwd_ke
 #pragma unroll
         for (int i = 0; i < 8; i += 4) {
           const float* s = h ? sb[k] : sw[k];
-          *reinterpret_cast<f32x4*>(join + wid * COLS + c[k] + i) = f32x4{s[i], s[i + 1], s[i + 2], s[i + 3]};
+          *reinterpret_cast<f32x4*>(join + (wid * (64 / LPR) + sub) * COLS + c[k] + i) =
+              f32x4{s[i], s[i + 1], s[i + 2], s[i + 3]};
         }
       __syncthreads();
       for (int n = threadIdx.x; n < N; n += ln_threads<WPR>()) {
         float s = 0.f;
 #pragma unroll
-        for (int v = 0; v < NW; ++v) s += join[v * COLS + n];
+        for (int v = 0; v < NV; ++v) s += join[v * COLS + n];
         pw[(size_t)h * N + n] = s;
       }
     }
@@ -410,16 +425,39 @@ __global__ __launch_bounds__(256) void ln_wgrad_wide_kernel(const T* __restrict_
   }
 }
 
-// the register tile of a width: (waves per row, chunks of 8 per lane); {0, 0}: the wide kernels
-struct LnPlan { int wpr, kc; };
+// the register tile of a width: (waves per row, chunks of 8 per lane, lanes of a wave per row); {0, 0, 0}: the wide kernels.
+// Rows of up to 256 columns share a wave, since a wave's latency is what a short row costs; forward / backward in us with a wave
+// per row and with the lanes below: 65536 x 64 bf16 18.4 / 25.9 and 5.5 / 10.3, x 128 19.4 / 30.9 and 8.0 / 15.6, x 256
+// 19.4 / 31.8 and 12.5 / 22.8, x 19 fp32 20.2 / 39.0 and 6.4 / 12.5
+struct LnPlan { int wpr, kc, lpr; };
 LnPlan ln_plan(int N) {
-  if (N <= 512) return {1, 1};
-  if (N <= 1024) return {1, 2};
-  if (N <= 2048) return {4, 1};
-  if (N <= 4096) return {4, 2};
-  if (N <= 8192) return {16, 1};
-  if (N <= 16384) return {16, 2};
-  return {0, 0};
+  if (N <= 64) return {1, 1, 8};
+  if (N <= 128) return {1, 1, 16};
+  if (N <= 256) return {1, 1, 32};
+  if (N <= 512) return {1, 1, 64};
+  if (N <= 1024) return {1, 2, 64};
+  if (N <= 2048) return {4, 1, 64};
+  if (N <= 4096) return {4, 2, 64};
+  if (N <= 8192) return {16, 1, 64};
+  if (N <= 16384) return {16, 2, 64};
+  return {0, 0, 0};
+}
+// f(integral_constant wpr, kc, lpr) for a plan with a register tile
+template <class F> int ln_dispatch(const LnPlan& p, F&& f) {
+#define LN_CASE(W, K, L)                    \
+  if (p.wpr == W && p.kc == K && p.lpr == L) \
+  return f(std::integral_constant<int, W>{}, std::integral_constant<int, K>{}, std::integral_constant<int, L>{})
+  LN_CASE(1, 1, 8);
+  LN_CASE(1, 1, 16);
+  LN_CASE(1, 1, 32);
+  LN_CASE(1, 1, 64);
+  LN_CASE(1, 2, 64);
+  LN_CASE(4, 1, 64);
+  LN_CASE(4, 2, 64);
+  LN_CASE(16, 1, 64);
+  LN_CASE(16, 2, 64);
+#undef LN_CASE
+  return (int)hipErrorInvalidValue;
 }
 
 constexpr int kMaxN = 1 << 30;   // column counters are 32 bits
@@ -430,7 +468,8 @@ constexpr int kMaxN = 1 << 30;   // column counters are 32 bits
 // four)
 int ln_bwd_grid(long M, int N) {
   const LnPlan p = ln_plan(N);
-  const long rows = p.wpr == 1 ? 8 : 2, want = (M + rows - 1) / rows, cap = (p.wpr == 4 && p.kc == 1 ? 4L : 3L) * crnn_cu_count();
+  const long rows = p.wpr == 1 ? 8 * (64 / p.lpr) : 2, want = (M + rows - 1) / rows;
+  const long cap = (p.wpr == 4 && p.kc == 1 ? 4L : 3L) * crnn_cu_count();
   return (int)(want < 1 ? 1 : want < cap ? want : cap);
 }
 int ln_wide_slices(long M) {
@@ -438,38 +477,21 @@ int ln_wide_slices(long M) {
   return (int)(s < 1 ? 1 : s < 64 ? s : 64);
 }
 
-template <typename T, int WPR, int KC>
-int ln_fwd_launch(const void* x, long ldx, const float* w, const float* b, void* y, long ldy, float* mean, float* rstd, long M,
-                  int N, float eps, hipStream_t st) {
-  long g = (M + ln_rpb<WPR>() - 1) / ln_rpb<WPR>();
-  const long cap = 8L * crnn_cu_count();
-  if (g > cap) g = cap;
-  hipLaunchKernelGGL((ln_fwd_kernel<T, WPR, KC>), dim3((int)g), dim3(ln_threads<WPR>()), 0, st, (const T*)x, ldx, w, b, (T*)y,
-                     ldy, mean, rstd, M, N, eps);
-  return (int)hipGetLastError();
-}
-
 template <typename T>
 int ln_fwd_t(const void* x, long ldx, const float* w, const float* b, void* y, long ldy, float* mean, float* rstd, long M, int N,
              float eps, hipStream_t st) {
   const LnPlan p = ln_plan(N);
-  if (p.wpr == 1 && p.kc == 1) return ln_fwd_launch<T, 1, 1>(x, ldx, w, b, y, ldy, mean, rstd, M, N, eps, st);
-  if (p.wpr == 1) return ln_fwd_launch<T, 1, 2>(x, ldx, w, b, y, ldy, mean, rstd, M, N, eps, st);
-  if (p.wpr == 4 && p.kc == 1) return ln_fwd_launch<T, 4, 1>(x, ldx, w, b, y, ldy, mean, rstd, M, N, eps, st);
-  if (p.wpr == 4) return ln_fwd_launch<T, 4, 2>(x, ldx, w, b, y, ldy, mean, rstd, M, N, eps, st);
-  if (p.wpr == 16 && p.kc == 1) return ln_fwd_launch<T, 16, 1>(x, ldx, w, b, y, ldy, mean, rstd, M, N, eps, st);
-  if (p.wpr == 16) return ln_fwd_launch<T, 16, 2>(x, ldx, w, b, y, ldy, mean, rstd, M, N, eps, st);
+  if (p.wpr)
+    return ln_dispatch(p, [&](auto W, auto K, auto L) {
+      constexpr int wpr = decltype(W)::value, kc = decltype(K)::value, lpr = decltype(L)::value, rpb = ln_rpb<wpr, lpr>();
+      const long g = (M + rpb - 1) / rpb, cap = 8L * crnn_cu_count();
+      hipLaunchKernelGGL((ln_fwd_kernel<T, wpr, kc, lpr>), dim3((int)(g < cap ? g : cap)), dim3(ln_threads<wpr>()), 0, st, (const T*)x,
+                         ldx, w, b, (T*)y, ldy, mean, rstd, M, N, eps);
+      return (int)hipGetLastError();
+    });
   const long cap = 2L * crnn_cu_count();
   hipLaunchKernelGGL(ln_fwd_wide_kernel<T>, dim3((int)(M < cap ? M : cap)), dim3(LW), 0, st, (const T*)x, ldx, w, b, (T*)y, ldy,
                      mean, rstd, M, N, eps);
-  return (int)hipGetLastError();
-}
-
-template <typename T, int WPR, int KC>
-int ln_bwd_launch(const void* dy, long lddy, const void* x, long ldx, const float* w, const float* mean, const float* rstd,
-                  const void* dres, long ldr, void* dx, long lddx, float* part, int G, long M, int N, hipStream_t st) {
-  hipLaunchKernelGGL((ln_bwd_kernel<T, WPR, KC>), dim3(G), dim3(ln_threads<WPR>()), 0, st, (const T*)dy, lddy, (const T*)x, ldx,
-                     w, mean, rstd, (const T*)dres, ldr, (T*)dx, lddx, part, M, N);
   return (int)hipGetLastError();
 }
 
@@ -482,11 +504,12 @@ int ln_bwd_t(const void* dy, long lddy, const void* x, long ldx, const float* w,
   int rc = 0, G = 0;
   if (M > 0 && p.wpr) {
     G = ln_bwd_grid(M, N);
-#define LN_GO(WPR, KC) ln_bwd_launch<T, WPR, KC>(dy, lddy, x, ldx, w, mean, rstd, dres, ldr, dx, lddx, part, G, M, N, st)
-    if (p.wpr == 1) rc = p.kc == 1 ? LN_GO(1, 1) : LN_GO(1, 2);
-    else if (p.wpr == 4) rc = p.kc == 1 ? LN_GO(4, 1) : LN_GO(4, 2);
-    else rc = p.kc == 1 ? LN_GO(16, 1) : LN_GO(16, 2);
-#undef LN_GO
+    rc = ln_dispatch(p, [&](auto W, auto K, auto L) {
+      constexpr int wpr = decltype(W)::value, kc = decltype(K)::value, lpr = decltype(L)::value;
+      hipLaunchKernelGGL((ln_bwd_kernel<T, wpr, kc, lpr>), dim3(G), dim3(ln_threads<wpr>()), 0, st, (const T*)dy, lddy, (const T*)x,
+                         ldx, w, mean, rstd, (const T*)dres, ldr, (T*)dx, lddx, part, M, N);
+      return (int)hipGetLastError();
+    });
   } else if (M > 0) {
     if (part) {   // before dx: dx may be dres, and neither dy nor x may be dx, so the order is free; kept first
       G = ln_wide_slices(M);

@@ -66,8 +66,9 @@ def ln_ref(x, w, b, dy, eps, dt):
     return (y, ey), (dx, edx), (dw, edw), (db, edb)
 
 
-LN_SIZES = [(1, 1), (3, 7), (1, 512), (5, 513), (17, 64), (1000, 512), (301, 768), (130, 1021), (9, 1024), (7, 1025), (6, 2048),
-            (33, 2049), (5, 4096), (3, 4097), (4, 8192), (3, 10007), (2, 16384), (3, 16385), (2, 40001), (6000, 33)]
+LN_SIZES = [(1, 1), (3, 7), (31, 8), (7, 65), (2003, 100), (1001, 128), (15, 129), (4099, 250), (3, 256), (2, 257),
+            (1, 512), (5, 513), (17, 64), (1000, 512), (301, 768), (130, 1021), (9, 1024), (7, 1025), (6, 2048), (33, 2049),
+            (5, 4096), (3, 4097), (4, 8192), (3, 10007), (2, 16384), (3, 16385), (2, 40001), (6000, 33)]
 
 
 @pytest.mark.parametrize("dt", TYPES)
@@ -137,7 +138,7 @@ def test_layer_norm_rows_do_not_mix():
 
 
 @pytest.mark.parametrize("dt", TYPES)
-@pytest.mark.parametrize("n", [96, 1500, 20000])
+@pytest.mark.parametrize("n", [40, 96, 200, 1500, 20000])
 def test_layer_norm_residual_gradient_and_accumulation(n, dt):
     """the C entry's dres (added before dx's one rounding, in place too) and accumulate"""
     g = gen(n)
