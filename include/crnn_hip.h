@@ -574,8 +574,9 @@ int crnn_layernorm_bwd(int dtype, const void* dy, long lddy, const void* x, long
  * y[M][N] = act(x[M][K] . w[N][K]^T + bias[N]) + res[M][N], act one of CRNN_ACT_*; accumulation, bias, activation and
  * residual in fp32, one rounding. x, w, y, res in dtype; bias fp32 (bias_f32 = 1) or dtype; bias, res may be NULL.
  * z (NULL: not stored) = the pre-activation in dtype, which the backward of gelu / silu / relu reads.
- * Any M >= 0, N, K >= 1 and element-aligned row strides: operands whose rows are not 16-byte aligned multiples of 8
- * are first copied into ws (crnn_linear_fwd_workspace bytes; 0 for aligned ones and for up to 32 rows). w stays under 2 GiB. */
+ * Any M >= 0, N, K >= 1 and element-aligned row strides. Rows are read as they lie, except that the largest bf16 products
+ * (256-row tiles that fill the CUs) first copy those that are not 16-byte aligned multiples of 8 into ws
+ * (crnn_linear_fwd_workspace bytes, else 0). w stays under 2 GiB. */
 #define CRNN_ACT_NONE 0
 #define CRNN_ACT_RELU 1
 #define CRNN_ACT_GELU 2 /* z Phi(z), the erf form */
@@ -599,8 +600,7 @@ int crnn_linear_bwd(int dtype, const void* dy, long lddy, const void* x, long ld
  * [0, D/2) forward and [D/2, D) backward in time (D even; the bidirectional encoder's [forward | reverse] rows). T, D <= 2^30.
  * lengths (NULL: all T) int32 [B], clamped to [0, T]: steps t >= lengths[b] are not read and get y = 0.
  * h0 (NULL: 0) fp32 [B][D]: the state before the first step; hT (NULL: not stored) fp32 [B][D]: the one after the last
- * (h0 where the length is 0; hT may be h0 where the
- * workspace is 0, e.g. for T <= 8). ckpt (NULL: inference): crnn_gated_scan_ckpt_bytes, fp32 states that the
+ * (h0 where the length is 0; hT may be h0 where the workspace is 0, e.g. for T <= 8). ckpt (NULL: inference): crnn_gated_scan_ckpt_bytes, fp32 states that the
  * backward recomputes h from. ws: crnn_gated_scan_workspace bytes (the segment summaries of long, few sequences). */
 size_t crnn_gated_scan_ckpt_bytes(int dtype, int B, int T, int D, int dir);
 size_t crnn_gated_scan_workspace(int dtype, int B, int T, int D, int dir);

@@ -18,10 +18,11 @@ def linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] =
     cores with fp32 accumulation), bias [N] in that dtype or fp32, residual [..., N] in that dtype (no broadcasting);
     activation "none", "relu", "gelu" (the erf form) or "silu". Bias, activation and residual are applied to the fp32
     sums and y is rounded once. Differentiable once in every tensor: the backward keeps the pre-activation in x's dtype,
-    d weight and d bias come in their own dtypes from fp32 sums in a fixed order. Any sizes >= 1 and any strides; rows that
-    are not 16-byte aligned multiples of 8 elements are copied into such ones first (not for up to 32 rows). weight, and each
-    row of x, stays under 2 GiB. Runs on x's device and its current torch stream; capturable. ValueError for arguments that
-    do not fit, RuntimeError for CPU tensors."""
+    d weight and d bias come in their own dtypes from fp32 sums in a fixed order. Any sizes >= 1 and any strides: rows are
+    read as they lie, except that the largest bf16 products copy rows that are not 16-byte aligned multiples of 8 elements into
+    such ones first. weight, and each row of x, stays under 2 GiB. Runs on x's device and its current torch stream; capturable
+    (a captured backward is refused while an eager graph of its leaves, built on the default stream, is alive). ValueError for
+    arguments that do not fit, RuntimeError for CPU tensors."""
     global _op
     if _op is None:
         _op = L.ops().linear.default

@@ -23,7 +23,8 @@ def gated_scan(f: torch.Tensor, v: torch.Tensor, h0: Optional[torch.Tensor] = No
     lengths[b] (clamped to 0 .. T) are not read, get y = 0 and no gradient, and leave the state as it is.
     return_state: -> (y, hT), hT fp32 [B, D] the state after the last step walked, from which the next stretch of the
     sequence continues. Differentiable once in f, v and h0. Runs on f's device and its current torch stream; capturable
-    where lengths is an int32 tensor on the device (another one is converted). ValueError for arguments that do not fit,
+    where lengths is an int32 tensor on the device (another one is converted); a captured backward is refused while an eager
+    graph of its leaves, built on the default stream, is alive. ValueError for arguments that do not fit,
     RuntimeError for CPU tensors."""
     global _op
     if _op is None:
@@ -39,5 +40,6 @@ def gated_scan(f: torch.Tensor, v: torch.Tensor, h0: Optional[torch.Tensor] = No
 
 def gated_scan_step(f: torch.Tensor, v: torch.Tensor, state: torch.Tensor, out_state: Optional[torch.Tensor] = None):
     """one step of running sequences: f, v [B, D] (fp32 or bf16), state fp32 [B, D] -> (y [B, D], next state). out_state: where the
-    next state is written (fp32 [B, D], contiguous); `state` itself updates it in place. Inference only."""
+    next state is written (fp32 [B, D], contiguous, over none of the inputs); `state` itself updates it in place. Inference
+    only."""
     return L.ops().gated_scan_step.default(f, v, state, out_state)

@@ -7,9 +7,11 @@
 // of the tensors' device and calls it. Its symbols are those of the libcrnn_hip.so that crnn_hip/_lib.py has loaded.
 #include <ATen/ATen.h>
 #include <c10/core/DeviceGuard.h>
+#include <c10/hip/HIPGraphsC10Utils.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/csrc/autograd/variable.h>
 #include <torch/library.h>
 
 #include "crnn_hip.h"
@@ -39,7 +41,16 @@ void check_type(const char* op, const char* name, const Tensor& t, at::ScalarTyp
                     t.scalar_type());
 }
 bool has(const OptTensor& t) { return t.has_value() && t->defined(); }
-bool wants_grad(const OptTensor& t) { return has(t) && t->requires_grad(); }
+// whether autograd has to record the call. Forward-mode tangents are refused: a plain call would drop them silently
+bool records(const char* op, std::initializer_list<OptTensor> ts) {
+  bool grad = false;
+  for (const OptTensor& t : ts) {
+    if (!has(t)) continue;
+    TORCH_CHECK(!t->_fw_grad(0).defined(), op, " has no forward-mode derivative");
+    grad = grad || t->requires_grad();
+  }
+  return grad && at::GradMode::is_enabled();
+}
 Tensor contiguous(const OptTensor& t) { return has(t) ? t->contiguous() : Tensor(); }
 void* ptr(const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
 float* fptr(const Tensor& t) { return (float*)ptr(t); }
@@ -69,6 +80,22 @@ Tensor floats(at::IntArrayRef shape, const Tensor& like) { return at::empty(shap
 
 void* stream(const Tensor& t) { return (void*)c10::hip::getCurrentHIPStream(t.get_device()).stream(); }
 void call(int rc, const char* name) { TORCH_CHECK(rc == 0, name, " failed (hip error ", rc, "): ", crnn_last_error_string()); }
+
+// A captured backward may not hand its gradients to a node of the default stream: autograd would order that stream behind the
+// captured one, which no capture allows, and torch does not survive it. Such a node is a leaf's accumulator that an eager graph,
+// built on the default stream and still alive, holds on to. Refused here, before autograd does it.
+void check_capture(const char* op) {
+  if (!c10::hip::getCurrentHIPStream().stream() || c10::hip::currentStreamCaptureStatusMayInitCtx() == c10::hip::CaptureStatus::None) return;
+  const auto node = torch::autograd::get_current_node();
+  if (!node) return;
+  for (size_t i = 0; i < node->num_outputs(); ++i) {
+    const auto& e = node->next_edge(i);
+    if (!e.is_valid() || !node->task_should_compute_output(i)) continue;
+    const auto s = e.function->stream();
+    TORCH_CHECK(!s || s->id() != 0, op, ": this backward is being captured into a graph, but an eager graph that was built on the default stream "
+                "and is still alive holds one of its inputs: drop that graph (its outputs and losses) before the capture");
+  }
+}
 
 // create_graph: the results refuse to be differentiated again
 variable_list once(const char* op, variable_list grads) {
@@ -120,6 +147,7 @@ struct LayerNormFn : public torch::autograd::Function<LayerNormFn> {
     {
       at::AutoDispatchBelowADInplaceOrView below;
       const c10::OptionalDeviceGuard guard(x.device());
+      check_capture("layer_norm");
       const auto shape = ctx->saved_data["shape"].toIntVector();
       const int64_t n = shape.back(), m = stats.numel() / 2, ld = ctx->saved_data["ld"].toInt();
       const int dt = dtype_code("layer_norm", x);
@@ -152,7 +180,7 @@ Tensor layer_norm(const Tensor& x, const OptTensor& weight, const OptTensor& bia
   TORCH_CHECK_VALUE(eps >= 0, "layer_norm: eps must be >= 0, got ", eps);
   require_device(x);
   const c10::OptionalDeviceGuard guard(x.device());
-  if (at::GradMode::is_enabled() && (x.requires_grad() || wants_grad(weight) || wants_grad(bias)))
+  if (records("layer_norm", {x, weight, bias}))
     return LayerNormFn::apply(x, weight, bias, eps);
   return layer_norm_run(rows(x), x.sizes(), contiguous(weight), contiguous(bias), eps, Tensor());
 }
@@ -203,6 +231,7 @@ struct LinearFn : public torch::autograd::Function<LinearFn> {
     {
       at::AutoDispatchBelowADInplaceOrView below;
       const c10::OptionalDeviceGuard guard(x.device());
+      check_capture("linear");
       if (need_x || need_w || need_b) {
         const int dt = dtype_code("linear", x), act = (int)ctx->saved_data["act"].toInt();
         const int64_t n = w.size(0), k = w.size(1), m = ctx->saved_data["m"].toInt(), ldx = ctx->saved_data["ldx"].toInt(),
@@ -246,7 +275,7 @@ Tensor linear(const Tensor& x, const Tensor& weight, const OptTensor& bias, int6
   }
   require_device(x);
   const c10::OptionalDeviceGuard guard(x.device());
-  if (at::GradMode::is_enabled() && (x.requires_grad() || weight.requires_grad() || wants_grad(bias) || wants_grad(residual)))
+  if (records("linear", {x, weight, bias, residual}))
     return LinearFn::apply(x, weight, bias, act, residual);
   return linear_run(rows(x), x.sizes(), rows(weight), contiguous(bias), (int)act, residual, Tensor());
 }
@@ -289,6 +318,7 @@ struct GatedScanFn : public torch::autograd::Function<GatedScanFn> {
     {
       at::AutoDispatchBelowADInplaceOrView below;
       const c10::OptionalDeviceGuard guard(f.device());
+      check_capture("gated_scan");
       const int dt = dtype_code("gated_scan", f);
       // only the final state was used: no upstream gradient for y
       const Tensor dy = g[0].defined() ? chan(g[0]) : at::zeros(f.sizes(), f.options());
@@ -308,6 +338,17 @@ struct GatedScanFn : public torch::autograd::Function<GatedScanFn> {
     return once("gated_scan", std::move(out));
   }
 };
+
+// no byte of a is a byte of b (taking each from its first to its last element)
+bool apart(const Tensor& a, const Tensor& b) {
+  if (!a.numel() || !b.numel()) return true;
+  auto end = [](const Tensor& t) {
+    int64_t n = 1;
+    for (int64_t i = 0; i < t.dim(); ++i) n += (t.size(i) - 1) * t.stride(i);
+    return (const char*)t.data_ptr() + n * t.element_size();
+  };
+  return end(a) <= (const char*)b.data_ptr() || end(b) <= (const char*)a.data_ptr();
+}
 
 void check_scan(const char* op, const Tensor& f, const Tensor& v, int64_t dims) {
   dtype_code(op, f);
@@ -335,7 +376,7 @@ std::tuple<Tensor, Tensor> gated_scan(const Tensor& f, const Tensor& v, const Op
   if (has(lengths)) {   // before the conversion: a 64-bit length must not wrap
     len = (lengths->scalar_type() == at::kLong ? lengths->clamp(0, T) : *lengths).to(f.options().dtype(at::kInt)).contiguous();
   }
-  if (at::GradMode::is_enabled() && (f.requires_grad() || v.requires_grad() || wants_grad(h0))) {
+  if (records("gated_scan", {f, v, h0})) {
     variable_list r = GatedScanFn::apply(f, v, h0, len, dir, state);
     return {r[0], state ? r[1] : Tensor()};
   }
@@ -348,21 +389,19 @@ std::tuple<Tensor, Tensor> gated_scan_step(const Tensor& f, const Tensor& v, con
   check_scan(op, f, v, 2);
   check(op, "state", state, f.sizes(), f);
   check_type(op, "state", state, at::kFloat, at::kFloat);
-  TORCH_CHECK(!(at::GradMode::is_enabled() && (f.requires_grad() || v.requires_grad() || state.requires_grad())),
+  TORCH_CHECK(!records(op, {f, v, state, out_state}),
               "gated_scan_step is inference only: use gated_scan(..., return_state=True) where gradients are needed");
   if (has(out_state)) {
     check(op, "out_state", *out_state, f.sizes(), f);
     check_type(op, "out_state", *out_state, at::kFloat, at::kFloat);
     TORCH_CHECK_VALUE(out_state->is_contiguous(), op, ": out_state must be contiguous");
-    const char *a = (const char*)out_state->data_ptr(), *b = (const char*)state.data_ptr();
-    const int64_t n = 4 * out_state->numel();
-    int64_t span = state.numel() ? 4 : 0;
-    if (span)
-      for (int64_t i = 0; i < 2; ++i) span += 4 * (state.size(i) - 1) * state.stride(i);
-    TORCH_CHECK_VALUE((a == b && state.is_contiguous()) || a >= b + span || b >= a + n, op, ": out_state overlaps state without being it");
+    TORCH_CHECK_VALUE((out_state->data_ptr() == state.data_ptr() && state.is_contiguous()) || apart(*out_state, state), op,
+                      ": out_state overlaps state without being it");
+    TORCH_CHECK_VALUE(apart(*out_state, f) && apart(*out_state, v), op, ": out_state overlaps f or v");
   }
   require_device(f);
   const c10::OptionalDeviceGuard guard(f.device());
+  if (has(out_state)) torch::autograd::impl::bump_version(*out_state);   // a graph that saved it has to notice
   Tensor out = has(out_state) ? *out_state : floats(f.sizes(), f);
   Tensor y = scan_run(chan(f.unsqueeze(1)), chan(v.unsqueeze(1)), state.contiguous(), Tensor(), 0, out, Tensor());
   return {y.squeeze(1), out};

@@ -66,6 +66,19 @@ def test_step_refuses_overlapping_states_and_gradients():
         crnn_hip.gated_scan_step(X.clone().requires_grad_(True), X, X)
 
 
+def test_step_refuses_an_output_that_is_an_input_or_a_leaf():
+    """out_state over f or v would be written while they are read; a leaf that wants a gradient is not written in place"""
+    buf = torch.zeros(60)
+    for i, lo in enumerate((0, 12, 23)):
+        f = buf[lo:lo + 24].view(4, 6)
+        with pytest.raises(ValueError, match="f or v"):
+            crnn_hip.gated_scan_step(*((f, X) if i % 2 else (X, f)), X, out_state=buf[:24].view(4, 6))
+    with pytest.raises(RuntimeError, match="HIP device"):      # beside it: the call gets as far as asking for a device
+        crnn_hip.gated_scan_step(buf[24:48].view(4, 6), X, X, out_state=buf[:24].view(4, 6))
+    with pytest.raises(RuntimeError, match="inference only"):
+        crnn_hip.gated_scan_step(X, X, X, out_state=torch.zeros(4, 6, requires_grad=True))
+
+
 @pytest.mark.parametrize("call", [
     lambda: crnn_hip.layer_norm(X),
     lambda: crnn_hip.linear(X, torch.zeros(3, 6)),

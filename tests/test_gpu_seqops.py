@@ -122,6 +122,23 @@ def test_layer_norm_layouts(dt):
     within("far", crnn_hip.layer_norm(far, w, b), *ln_ref(far, w, b, torch.zeros_like(far), 1e-5, dt)[0])
 
 
+@pytest.mark.parametrize("n", [5, 60, 100, 256])
+def test_layer_norm_rows_of_a_wave_do_not_mix(n):
+    """narrow rows share a wave: a NaN or infinity stays in its own, forward and backward"""
+    g = gen(n)
+    x, dy = randn(g, 37, n), randn(g, 37, n)
+    keep = [i for i in range(37) if i not in (3, 7, 36)]
+
+    def run(x):
+        lx = x.clone().requires_grad_(True)
+        y = crnn_hip.layer_norm(lx)
+        return y.detach(), torch.autograd.grad(y, lx, dy)[0]
+    x2 = x.clone()
+    x2[3, n - 1], x2[7, 1], x2[36, 0] = float("nan"), float("inf"), float("-inf")
+    for a, b in zip(run(x), run(x2)):
+        assert torch.equal(a[keep], b[keep]) and torch.isnan(b[[3, 7, 36]]).all()
+
+
 def test_layer_norm_rows_do_not_mix():
     """a NaN or infinite row stays its own; the strided output of a wider buffer's neighbours is not touched"""
     g = gen(6)
@@ -648,6 +665,60 @@ def test_capture_and_replay():
             torch.cuda.synchronize()
             for a, b in zip([o.clone() for o in out], step()):
                 assert torch.equal(a, b), i
+
+
+def seq_calls(g):
+    """name -> (function of a leaf, the leaf) of each operator"""
+    w, h = randn(g, 24, 16), randn(g, 2, 16)
+    return {"layer_norm": (lambda x: crnn_hip.layer_norm(x), randn(g, 2, 5, 16)),
+            "linear": (lambda x: crnn_hip.linear(x, w, activation="gelu"), randn(g, 2, 5, 16)),
+            "gated_scan": (lambda x: crnn_hip.gated_scan(x, x, h0=h), randn(g, 2, 5, 16))}
+
+
+@pytest.mark.parametrize("op", ["layer_norm", "linear", "gated_scan"])
+def test_forward_mode_is_refused(op):
+    """a tangent would be dropped without a word"""
+    import torch.autograd.forward_ad as fwAD
+    fn, x = seq_calls(gen(62))[op]
+    with fwAD.dual_level():
+        with pytest.raises(RuntimeError, match="forward-mode"):
+            fn(fwAD.make_dual(x, torch.ones_like(x)))
+        with torch.no_grad(), pytest.raises(RuntimeError, match="forward-mode"):
+            fn(fwAD.make_dual(x, torch.ones_like(x)))
+
+
+def test_step_in_place_is_noticed_by_autograd():
+    """a graph that saved the state before it was stepped in place must not run on with the new one"""
+    g = gen(63)
+    f, w, state = randn(g, 3, 8), randn(g, 3, 8).requires_grad_(True), randn(g, 3, 8)
+    loss = (state * w).sum()
+    crnn_hip.gated_scan_step(f, f, state, out_state=state)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        loss.backward()
+
+
+@pytest.mark.parametrize("op", ["layer_norm", "linear", "gated_scan"])
+def test_captured_backward_beside_an_eager_graph_of_the_leaf(op):
+    """an eager graph of the same leaf, built on the default stream and still alive: the captured backward is refused before
+    autograd orders the default stream behind the capture; without that graph the same capture is made"""
+    g = gen(64)
+    fn, x = seq_calls(g)[op]
+    x.requires_grad_(True)
+    dy = randn(g, *fn(x).shape)
+    (want,) = torch.autograd.grad(fn(x), x, dy)
+    held = fn(x)
+    with pytest.raises(RuntimeError, match="eager graph"):
+        with torch.cuda.graph(torch.cuda.CUDAGraph()):
+            torch.autograd.grad(fn(x), x, dy)
+    del held
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        (got,) = torch.autograd.grad(fn(x), x, dy)
+    for _ in range(3):
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(got, want)
+        got.zero_()
 
 
 def test_rows_past_32_bits():
