@@ -40,7 +40,11 @@ class GLRStack:
 
     # ---------------------------------------------------------------- pieces
     def _bytes(self, n):
-        return self.eng.ws.get(f"glr.ws.{n}", (n,), torch.uint8) if n else None
+        """scratch of one kernel call; the calls follow each other on one stream, so they share the largest asked for so far"""
+        have = self.eng.ws.bufs.get("glr.ws")
+        if n and (have is None or have.numel() < n):
+            have = self.eng.ws.get("glr.ws", (n,), torch.uint8)
+        return have if n else None
 
     def _norm(self, l, name, x, M, keep):
         e = self.eng

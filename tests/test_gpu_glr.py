@@ -76,6 +76,29 @@ def test_stack_matches_fp64(hidden, B, T, dtype, tol):
 
 
 @pytest.mark.gpu
+def test_lines_of_many_lengths_share_the_scratch():
+    """batches of other geometries: the same results as a fresh engine's, and one scratch buffer, not one a size"""
+    def engine():
+        m = make(64, torch.bfloat16).to(DEV).train()
+        m.flatten_parameters_()
+        return m, m._engine_for(torch.zeros(1, 3, 32, 8, device=DEV))
+    m, eng = engine()
+    g = torch.Generator(device=DEV).manual_seed(10)
+    grads, _, _ = m._grad_views()
+    for B, T in ((2, 40), (1, 700), (5, 9), (2, 40)):
+        x, dout = torch.randn(B, T, 512, generator=g, device=DEV), torch.randn(B, T, 64, generator=g, device=DEV)
+        y, dx = eng.bilstm_stack(x, dout, grads)
+        m2, fresh = engine()
+        grads2, _, _ = m2._grad_views()
+        y2, dx2 = fresh.bilstm_stack(x, dout, grads2)
+        assert torch.equal(y, y2) and torch.equal(dx, dx2)
+        for k in grads:
+            if k.startswith("enc_rnn."):
+                assert torch.equal(grads[k], grads2[k]), k
+    assert len([k for k in eng.ws.bufs if k.startswith("glr.ws")]) == 1
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 def test_model_trains_end_to_end(dtype):
     """the whole model: every parameter gets its gradient, a second backward accumulates, eval agrees with train"""
