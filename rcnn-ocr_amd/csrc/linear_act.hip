@@ -298,8 +298,9 @@ size_t up256(size_t n) { return (n + 255) & ~(size_t)255; }
 // 86 us at 2 rounds of the former, 94 at 3 of the latter; 8192 x 1024 x 512: 24 at half a round, 20 at a whole one).
 // Else 64 x 64 register-staged tiles where there is one per CU (4096 x 512 x 512: 12.8 us; 256 x 128 tiles 19.8, 128 x 128
 // 19.8, 32 x 32 13.6), else 32 x 32 (500 x 520 x 512: 8.0 against 9.1). fp32 (exact-fp32 MFMA, 1/16 of the bf16 rate): 64 x 64
-// at four per CU or more (8192 x 1024 x 512: 84.8 us, 128 x 128 83.0, 32 x 32 101), else 32 x 32 with 64-deep stages
-// (1032 x 1024 x 512: 22.6 against 27.4 of 64 x 64; 304 x 520 x 1000: 13.1 against 28.7).
+// at two per CU or more (8192 x 1024 x 512: 84.8 us, 128 x 128 83.0, 32 x 32 101; forward and input gradient of 4096 x 512 x 512
+// 25.9 and 22.9, 32 x 32 28.2 and 28.6), else 32 x 32 with 64-deep stages (1032 x 1024 x 512: 19.7 against 24.4 of 64 x 64;
+// 304 x 520 x 1000: 13.1 against 28.7).
 // 0: register-staged, else the columns of the deep kernel's tile
 int deep_tile(int es, long M, int N, int K) {
   const long cu = crnn_cu_count(), t256 = (M + 255) / 256 * ((N + 255) / 256), t128 = (M + 255) / 256 * ((N + 127) / 128);
@@ -309,7 +310,7 @@ int deep_tile(int es, long M, int N, int K) {
 template <typename T, int ACT, class LA, class LB>
 int staged_run(const LA& la, const LB& lb, const ActEpi<T, ACT>& ep, int M, int N, int K, hipStream_t st) {
   const long cu = crnn_cu_count(), t64 = (long)((M + 63) / 64) * ((N + 63) / 64);
-  if (t64 >= (sizeof(T) == 2 ? cu : 4 * cu)) return launch<T, 64, 64>(la, lb, ep, M, N, K, 1, st);
+  if (t64 >= (sizeof(T) == 2 ? cu : 2 * cu)) return launch<T, 64, 64>(la, lb, ep, M, N, K, 1, st);
   return launch<T, 32, 32, 64>(la, lb, ep, M, N, K, 1, st);
 }
 template <typename T, int ACT, class LA, class LB>
@@ -563,7 +564,8 @@ int dz_slices(long M, int N) {
 // 256 x 256 kernel at one workgroup per CU if a split keeps 1024 rows (768 x 1536 over 32768: 75 us in 14 splits; 128 x 128
 // 100 in 7), else 128 x 128 at two per CU if it keeps 512 (1024 x 512 over 8192: 21 in 16; 64 x 64 23, 256 x 256 23 in 32), else
 // 64 x 64 (512 x 512 over 4096: 10.9 in 8; 128 x 128 11.6). fp32: 64 x 64 at four per CU (1024 x 512 over 1032: 19.9; 128 x 128
-// 30.7).
+// 30.7) of 256 rows or more, of 128 where that leaves fewer than two (512 x 520 over 500: 17.1 and 10.8; 700 x 300 over 2000:
+// 27.3 and 23.8; 1024 x 512 over 1024, which has two: 21.7 and 24.3).
 struct DwPlan { int tile, splits; };
 DwPlan dw_plan(int es, int Nr, int Kc, long rows) {
   const long cu = crnn_cu_count();
@@ -578,7 +580,8 @@ DwPlan dw_plan(int es, int Nr, int Kc, long rows) {
     if (s128 >= 1 && rows / s128 >= 512) return {128, split(s128, 512)};
     return {64, split(2 * cu / tiles(64), 256)};
   }
-  return {64, split(4 * cu / tiles(64), 256)};
+  const int s = split(4 * cu / tiles(64), 256);
+  return {64, s * tiles(64) < 2 * cu ? split(4 * cu / tiles(64), 128) : s};
 }
 
 // the layout of crnn_linear_bwd's workspace
