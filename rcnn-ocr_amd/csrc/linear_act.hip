@@ -503,29 +503,33 @@ struct SlabEpi {
   __device__ __forceinline__ void stats(int, int, f32x4, f32x4) const {}
 };
 // the last pass of the backward, one launch: workgroups [0, wblocks) add the S slabs into dw [N][K], the others G partial rows
-// of the column sums into db (64 columns each, 4 row lanes); every sum in a fixed order
+// of the column sums into db (32 columns each, 8 row lanes); every sum in a fixed order
 template <typename OW, typename OB>
 __global__ __launch_bounds__(256) void reduce_kernel(const float* __restrict__ slab, int S, int Nr, int Kc, OW* __restrict__ dw,
                                                      int wblocks, const float* __restrict__ part, int G, OB* __restrict__ db, int N,
                                                      int K, int accumulate) {
   if ((int)blockIdx.x >= wblocks) {
-    __shared__ float red[4][64];
-    const int col = threadIdx.x & 63, rl = threadIdx.x >> 6, n = ((int)blockIdx.x - wblocks) * 64 + col;
+    __shared__ float red[8][32];
+    const int col = threadIdx.x & 31, rl = threadIdx.x >> 5, n = ((int)blockIdx.x - wblocks) * 32 + col;
     float s = 0.f;
     if (n < N) {
       int g = rl;
-      for (; g + 15 * 4 < G; g += 16 * 4) {
+      for (; g + 15 * 8 < G; g += 16 * 8) {
         float v[16];
 #pragma unroll
-        for (int u = 0; u < 16; ++u) v[u] = part[(size_t)(g + 4 * u) * N + n];
+        for (int u = 0; u < 16; ++u) v[u] = part[(size_t)(g + 8 * u) * N + n];
 #pragma unroll
         for (int u = 0; u < 16; ++u) s += v[u];
       }
-      for (; g < G; g += 4) s += part[(size_t)g * N + n];
+      for (; g < G; g += 8) s += part[(size_t)g * N + n];
     }
     red[rl][col] = s;
     __syncthreads();
-    if (rl == 0 && n < N) put<OB>(db + n, s + red[1][col] + red[2][col] + red[3][col], accumulate);
+    if (rl == 0 && n < N) {
+#pragma unroll
+      for (int r = 1; r < 8; ++r) s += red[r][col];
+      put<OB>(db + n, s, accumulate);
+    }
     return;
   }
   const long total = (long)Nr * Kc;
@@ -696,7 +700,7 @@ int bwd_t(const BwdPlan& p, const void* dy, long lddy, const void* x, long ldx, 
     }
   }
   if (dw || db) {
-    const int wb = dw ? grid_for((long)p.N8 * p.K8 / 4, 256, 2048) : 0, bb = db ? (N + 63) / 64 : 0, G = M > 0 ? p.slices : 0;
+    const int wb = dw ? grid_for((long)p.N8 * p.K8 / 4, 256, 2048) : 0, bb = db ? (N + 31) / 32 : 0, G = M > 0 ? p.slices : 0;
     auto go = [&](auto ow, auto ob) {
       typedef decltype(ow) OW;
       typedef decltype(ob) OB;
