@@ -687,6 +687,69 @@ def test_forward_mode_is_refused(op):
             fn(fwAD.make_dual(x, torch.ones_like(x)))
 
 
+@pytest.mark.parametrize("op", ["layer_norm", "linear", "gated_scan"])
+@pytest.mark.parametrize("dt", TYPES)
+def test_every_subset_of_gradients(op, dt):
+    """whichever inputs want a gradient, each gets what it gets when all do; under no_grad and inference_mode the same output"""
+    import itertools
+    g = gen(65)
+    if op == "layer_norm":
+        args, fn = [randn(g, 40, 72, dtype=dt), randn(g, 72), randn(g, 72)], crnn_hip.layer_norm
+    elif op == "linear":
+        args = [randn(g, 40, 72, dtype=dt), randn(g, 48, 72, dtype=dt), randn(g, 48), randn(g, 40, 48, dtype=dt)]
+        fn = lambda x, w, b, r: crnn_hip.linear(x, w, b, activation="silu", residual=r)  # noqa: E731
+    else:
+        args = [randn(g, 3, 20, 72, dtype=dt), randn(g, 3, 20, 72, dtype=dt), randn(g, 3, 72)]
+        fn = lambda f, v, h: crnn_hip.gated_scan(f, v, h0=h)  # noqa: E731
+    every = [a.clone().requires_grad_(True) for a in args]
+    y = fn(*every)
+    dy = randn(g, *y.shape, dtype=dt)
+    want = torch.autograd.grad(y, every, dy)
+    for k in range(1, len(args)):
+        for pick in itertools.combinations(range(len(args)), k):
+            leaves = [a.clone().requires_grad_(i in pick) for i, a in enumerate(args)]
+            out = fn(*leaves)
+            got = torch.autograd.grad(out, [leaves[i] for i in pick], dy)
+            assert torch.equal(out, y)
+            for i, a in zip(pick, got):
+                assert torch.equal(a, want[i]), (pick, i)
+    for mode in (torch.no_grad, torch.inference_mode):
+        with mode():
+            assert torch.equal(fn(*every), y)
+
+
+def test_two_threads_at_once():
+    """calls from two host threads, each on a stream of its own"""
+    import threading
+    g = gen(66)
+    w, b = randn(g, 96, 64, dtype=torch.bfloat16), randn(g, 96)
+    xs = [randn(g, 2, 150, 64, dtype=torch.bfloat16) for _ in range(2)]
+
+    def work(x):
+        lx = x.clone().requires_grad_(True)
+        y = crnn_hip.linear(crnn_hip.layer_norm(lx), w, b, activation="gelu")
+        y = crnn_hip.gated_scan(y, y, direction="both")
+        return y.detach(), torch.autograd.grad(y.float().square().sum(), lx)[0]
+    want, got = [work(x) for x in xs], [[], []]
+    torch.cuda.synchronize()
+
+    def run(i):
+        s = torch.cuda.Stream()
+        with torch.cuda.stream(s):
+            for _ in range(5):
+                got[i].append(work(xs[i]))
+        s.synchronize()
+    threads = [threading.Thread(target=run, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    for i in range(2):
+        assert len(got[i]) == 5
+        for r in got[i]:
+            assert torch.equal(r[0], want[i][0]) and torch.equal(r[1], want[i][1])
+
+
 def test_step_in_place_is_noticed_by_autograd():
     """a graph that saved the state before it was stepped in place must not run on with the new one"""
     g = gen(63)
