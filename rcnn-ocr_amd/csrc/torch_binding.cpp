@@ -81,6 +81,40 @@ Tensor floats(at::IntArrayRef shape, const Tensor& like) { return at::empty(shap
 void* stream(const Tensor& t) { return (void*)c10::hip::getCurrentHIPStream(t.get_device()).stream(); }
 void call(int rc, const char* name) { TORCH_CHECK(rc == 0, name, " failed (hip error ", rc, "): ", crnn_last_error_string()); }
 
+// What the backward reads goes through autograd's saved tensors, and a saved-tensor hook (offloading to the host and back,
+// torch.autograd.graph.save_on_cpu) may give back another layout than it took. So nothing about a layout is kept beside them: strides are
+// read from what comes back, and a tensor of another shape, type or device is refused.
+void save(AutogradContext* ctx, const variable_list& ts) {
+  std::vector<int64_t> meta;
+  for (const Tensor& t : ts) {
+    meta.push_back(t.defined() ? t.dim() : -1);
+    if (!t.defined()) continue;
+    meta.push_back((int64_t)t.scalar_type());
+    meta.push_back(t.get_device());
+    meta.insert(meta.end(), t.sizes().begin(), t.sizes().end());
+  }
+  ctx->save_for_backward(ts);
+  ctx->saved_data["meta"] = std::move(meta);
+}
+variable_list saved(const char* op, AutogradContext* ctx) {
+  variable_list ts = ctx->get_saved_variables();
+  const auto meta = ctx->saved_data["meta"].toIntVector();
+  const int64_t* p = meta.data();
+  for (const Tensor& t : ts) {
+    const int64_t dim = *p++;
+    TORCH_CHECK(t.defined() == (dim >= 0), op, ": a saved-tensor hook gave back ", t.defined() ? "a tensor for none" : "no tensor");
+    if (dim < 0) continue;
+    const auto type = (at::ScalarType)p[0];
+    const int64_t dev = p[1];
+    const at::IntArrayRef shape(p + 2, dim);
+    p += 2 + dim;
+    TORCH_CHECK(t.is_cuda() && t.get_device() == dev && t.scalar_type() == type && t.sizes() == shape && t.layout() == at::kStrided, op,
+                ": a saved-tensor hook gave back a ", t.scalar_type(), " tensor of shape ", t.sizes(), " on ", t.device(), " for a ", type,
+                " one of shape ", shape, " on device ", dev);
+  }
+  return ts;
+}
+
 // A captured backward may not hand its gradients to a node of the default stream: autograd would order that stream behind the
 // captured one, which no capture allows, and torch does not survive it. Such a node is a leaf's accumulator that an eager graph,
 // built on the default stream and still alive, holds on to. Refused here, before autograd does it.
@@ -129,16 +163,14 @@ struct LayerNormFn : public torch::autograd::Function<LayerNormFn> {
     const Tensor w = contiguous(weight), b = contiguous(bias);
     Tensor stats = floats({2 * r.m}, x);   // mean, then rstd of every row
     Tensor y = layer_norm_run(r, x.sizes(), w, b, eps, stats);
-    ctx->save_for_backward({r.t, w, stats});
-    ctx->saved_data["shape"] = x.sizes().vec();
-    ctx->saved_data["ld"] = r.ld;
+    save(ctx, {r.t, w, stats});
     ctx->saved_data["w"] = has(weight);
     ctx->saved_data["b"] = has(bias);
     return y;
   }
   static variable_list backward(AutogradContext* ctx, variable_list g) {
-    const auto saved = ctx->get_saved_variables();
-    const Tensor &x = saved[0], &w = saved[1], &stats = saved[2];
+    const auto kept = saved("layer_norm", ctx);
+    const Tensor& x = kept[0];
     const bool has_w = ctx->saved_data["w"].toBool(), has_b = ctx->saved_data["b"].toBool();
     size_t e = 0;
     const bool need_x = ctx->needs_input_grad(e++);
@@ -148,17 +180,17 @@ struct LayerNormFn : public torch::autograd::Function<LayerNormFn> {
       at::AutoDispatchBelowADInplaceOrView below;
       const c10::OptionalDeviceGuard guard(x.device());
       check_capture("layer_norm");
-      const auto shape = ctx->saved_data["shape"].toIntVector();
-      const int64_t n = shape.back(), m = stats.numel() / 2, ld = ctx->saved_data["ld"].toInt();
+      const Rows xr = rows(x), dy = rows(g[0]);
+      const Tensor w = contiguous(kept[1]), stats = kept[2].contiguous();
+      const int64_t n = x.size(-1), m = stats.numel() / 2;
       const int dt = dtype_code("layer_norm", x);
-      const Rows dy = rows(g[0]);
-      if (need_x) out[0] = at::empty(shape, x.options());
+      if (need_x) out[0] = at::empty(x.sizes(), x.options());
       if (need_w) out[1] = floats({n}, x);
       if (need_b) out[2] = floats({n}, x);
       const size_t need = need_w || need_b ? crnn_layernorm_bwd_workspace(dt, m, (int)n) : 0;
       const Tensor ws = bytes(need, x);
       float* s = fptr(stats);
-      call(crnn_layernorm_bwd(dt, ptr(dy.t), dy.ld, ptr(x), ld, fptr(w), s, s + m, nullptr, 0, ptr(out[0]), n, fptr(out[1]), fptr(out[2]), 0,
+      call(crnn_layernorm_bwd(dt, ptr(dy.t), dy.ld, ptr(xr.t), xr.ld, fptr(w), s, s + m, nullptr, 0, ptr(out[0]), n, fptr(out[1]), fptr(out[2]), 0,
                               fptr(ws), need, m, (int)n, stream(x)),
            "crnn_layernorm_bwd");
     }
@@ -209,19 +241,15 @@ struct LinearFn : public torch::autograd::Function<LinearFn> {
     const Rows r = rows(x), w = rows(weight);
     const Tensor z = act ? at::empty({r.m, weight.size(0)}, x.options()) : Tensor();   // the pre-activation
     Tensor y = linear_run(r, x.sizes(), w, contiguous(bias), (int)act, residual, z);
-    ctx->save_for_backward({r.t, w.t, z});
-    ctx->saved_data["shape"] = x.sizes().vec();
-    ctx->saved_data["m"] = r.m;
-    ctx->saved_data["ldx"] = r.ld;
-    ctx->saved_data["ldw"] = w.ld;
+    save(ctx, {r.t, w.t, z});
     ctx->saved_data["act"] = act;
     ctx->saved_data["b"] = has(bias) ? (bias->scalar_type() == at::kFloat ? 2 : 1) : 0;   // 2: fp32
     ctx->saved_data["r"] = has(residual);
     return y;
   }
   static variable_list backward(AutogradContext* ctx, variable_list g) {
-    const auto saved = ctx->get_saved_variables();
-    const Tensor &x = saved[0], &w = saved[1], &z = saved[2];
+    const auto kept = saved("linear", ctx);
+    const Tensor &x = kept[0], &w = kept[1];
     const int64_t bias = ctx->saved_data["b"].toInt();
     size_t e = 0;
     const bool need_x = ctx->needs_input_grad(e++), need_w = ctx->needs_input_grad(e++);
@@ -234,15 +262,16 @@ struct LinearFn : public torch::autograd::Function<LinearFn> {
       check_capture("linear");
       if (need_x || need_w || need_b) {
         const int dt = dtype_code("linear", x), act = (int)ctx->saved_data["act"].toInt();
-        const int64_t n = w.size(0), k = w.size(1), m = ctx->saved_data["m"].toInt(), ldx = ctx->saved_data["ldx"].toInt(),
-                      ldw = ctx->saved_data["ldw"].toInt();
-        const Rows dy = rows(g[0]);
-        if (need_x) out[0] = at::empty(ctx->saved_data["shape"].toIntVector(), x.options());
+        const Rows xr = rows(x), wr = rows(w), dy = rows(g[0]);
+        const Tensor z = contiguous(kept[2]);
+        const int64_t n = w.size(0), k = w.size(1), m = xr.m;
+        if (need_x) out[0] = at::empty(x.sizes(), x.options());
         if (need_w) out[1] = at::empty({n, k}, w.options());
         if (need_b) out[2] = bias == 2 ? floats({n}, x) : at::empty({n}, x.options());
-        const size_t need = crnn_linear_bwd_workspace(dt, ptr(dy.t), dy.ld, ptr(x), ldx, ptr(w), ldw, act, need_x, need_w, need_b, m, (int)n, (int)k);
+        const size_t need = crnn_linear_bwd_workspace(dt, ptr(dy.t), dy.ld, ptr(xr.t), xr.ld, ptr(wr.t), wr.ld, act, need_x, need_w, need_b, m,
+                                                      (int)n, (int)k);
         const Tensor ws = bytes(need, x);
-        call(crnn_linear_bwd(dt, ptr(dy.t), dy.ld, ptr(x), ldx, ptr(w), ldw, ptr(z), n, act, ptr(out[0]), k, ptr(out[1]),
+        call(crnn_linear_bwd(dt, ptr(dy.t), dy.ld, ptr(xr.t), xr.ld, ptr(wr.t), wr.ld, ptr(z), n, act, ptr(out[0]), k, ptr(out[1]),
                              w.scalar_type() == at::kFloat, ptr(out[2]), bias == 2, 0, ptr(ws), need, m, (int)n, (int)k, stream(x)),
              "crnn_linear_bwd");
       }
@@ -301,7 +330,7 @@ struct GatedScanFn : public torch::autograd::Function<GatedScanFn> {
     const Tensor ckpt = bytes(crnn_gated_scan_ckpt_bytes(dtype_code("gated_scan", f), B, T, D, (int)dir), f);   // the backward starts from it
     const Tensor hT = state ? floats({B, D}, f) : Tensor();
     Tensor y = scan_run(f, v, contiguous(h0), len, (int)dir, hT, ckpt);
-    ctx->save_for_backward({f, v, len, ckpt});
+    save(ctx, {f, v, len, ckpt});
     ctx->saved_data["dir"] = dir;
     ctx->saved_data["h0"] = has(h0);
     ctx->set_materialize_grads(false);
@@ -309,16 +338,16 @@ struct GatedScanFn : public torch::autograd::Function<GatedScanFn> {
     return {y};
   }
   static variable_list backward(AutogradContext* ctx, variable_list g) {
-    const auto saved = ctx->get_saved_variables();
-    const Tensor &f = saved[0], &v = saved[1], &len = saved[2], &ckpt = saved[3];
-    const int dir = (int)ctx->saved_data["dir"].toInt(), B = (int)f.size(0), T = (int)f.size(1), D = (int)f.size(2);
+    const auto kept = saved("gated_scan", ctx);
+    const int dir = (int)ctx->saved_data["dir"].toInt(), B = (int)kept[0].size(0), T = (int)kept[0].size(1), D = (int)kept[0].size(2);
     const bool need_f = ctx->needs_input_grad(0), need_v = ctx->needs_input_grad(1);
     const bool need_h = ctx->saved_data["h0"].toBool() && ctx->needs_input_grad(2);
     variable_list out(6);
     {
       at::AutoDispatchBelowADInplaceOrView below;
-      const c10::OptionalDeviceGuard guard(f.device());
+      const c10::OptionalDeviceGuard guard(kept[0].device());
       check_capture("gated_scan");
+      const Tensor f = chan(kept[0]), v = chan(kept[1]), len = contiguous(kept[2]), ckpt = kept[3].contiguous();
       const int dt = dtype_code("gated_scan", f);
       // only the final state was used: no upstream gradient for y
       const Tensor dy = g[0].defined() ? chan(g[0]) : at::zeros(f.sizes(), f.options());

@@ -810,3 +810,61 @@ def test_rows_past_32_bits():
         assert torch.equal(crnn_hip.gated_scan(f, f), crnn_hip.gated_scan(c, c))
     del big
     torch.cuda.empty_cache()
+
+
+# ------------------------------------------------------------------------------------------------ saved-tensor hooks
+def strided_calls(g, dt):
+    """operator -> (function, leaves), every operand a view whose rows lie apart; the values depend on g alone"""
+    wide = lambda *s: randn(g, *s[:-1], 3 * s[-1] + 5, dtype=dt)[..., 1:1 + s[-1]]  # noqa: E731
+    return {"layer_norm": (crnn_hip.layer_norm, [wide(6, 7, 70), randn(g, 70), randn(g, 70)]),
+            "linear": (lambda x, w, b, r: crnn_hip.linear(x, w, b, activation="gelu", residual=r),
+                       [wide(6, 7, 72), wide(48, 72), randn(g, 48), wide(6, 7, 48)]),
+            "gated_scan": (lambda f, v, h: crnn_hip.gated_scan(f, v, h0=h, lengths=torch.tensor([9, 4, 0], dtype=torch.int32, device=DEV)),
+                           [wide(3, 9, 66), wide(3, 9, 66), randn(g, 3, 66)])}
+
+
+def spread_out(t):
+    """the same values, every element two apart"""
+    return torch.stack([t, t], -1)[..., 0]
+
+
+def turned(t):
+    """the same values, the last axis outermost in memory"""
+    return t.movedim(-1, 0).contiguous().movedim(0, -1) if t.dim() else t.clone()
+
+
+@pytest.mark.parametrize("dt", TYPES)
+@pytest.mark.parametrize("op", ["layer_norm", "linear", "gated_scan"])
+@pytest.mark.parametrize("how", ["host", "compact", "spread", "turned"])
+def test_saved_tensor_hooks_may_change_layouts(op, how, dt):
+    """what the backward reads comes back from the host compact, or in other strides: the same gradients, bit for bit"""
+    fn, args = strided_calls(gen(81), dt)[op]
+    leaves = [a.detach().requires_grad_(True) for a in args]
+    assert any(not a.is_contiguous() for a in leaves)
+    y = fn(*leaves)
+    dy = randn(gen(82), *y.shape, dtype=dt)
+    want = torch.autograd.grad(y, leaves, dy)
+    seen = []
+    hooks = {"host": lambda: torch.autograd.graph.save_on_cpu(),
+             "compact": lambda: torch.autograd.graph.saved_tensors_hooks(lambda t: t.clone(memory_format=torch.contiguous_format), lambda t: t),
+             "spread": lambda: torch.autograd.graph.saved_tensors_hooks(lambda t: t, lambda t: seen.append(1) or spread_out(t)),
+             "turned": lambda: torch.autograd.graph.saved_tensors_hooks(lambda t: t, lambda t: seen.append(1) or turned(t))}[how]
+    with hooks():
+        y2 = fn(*leaves)
+    assert torch.equal(y2, y)
+    for a, b in zip(torch.autograd.grad(y2, leaves, dy), want):
+        assert torch.equal(a, b)
+    assert seen or how in ("host", "compact")
+
+
+@pytest.mark.parametrize("op", ["layer_norm", "linear", "gated_scan"])
+@pytest.mark.parametrize("what", ["host", "type", "shape"])
+def test_saved_tensors_that_do_not_fit_are_refused(op, what):
+    """a hook that gives back a tensor of another device, type or shape: an error before anything is launched"""
+    fn, args = strided_calls(gen(83), torch.float32)[op]
+    leaves = [a.detach().requires_grad_(True) for a in args]
+    change = {"host": lambda t: t.cpu(), "type": lambda t: t.double(), "shape": lambda t: t[..., :-1]}[what]
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: t, change):
+        y = fn(*leaves)
+    with pytest.raises(RuntimeError, match=f"{op}: a saved-tensor hook gave back"):
+        torch.autograd.grad(y, leaves, torch.ones_like(y))
