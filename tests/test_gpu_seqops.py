@@ -868,3 +868,194 @@ def test_saved_tensors_that_do_not_fit_are_refused(op, what):
         y = fn(*leaves)
     with pytest.raises(RuntimeError, match=f"{op}: a saved-tensor hook gave back"):
         torch.autograd.grad(y, leaves, torch.ones_like(y))
+
+
+# ------------------------------------------------------------------------------------------------ the plans of large calls
+def linear_plan(m, k, n):
+    """(columns of the forward's deep tiles, of the input gradient's, tile of the weight gradient, its splits) of a bf16 product of
+    whole vectors, as far as the workspaces tell: a deep kernel copies an operand that is not 16-byte aligned, the others read it
+    as it lies, and the weight gradient has a slab a split. 256 or 128 columns by the weighted rounds of the tiles"""
+    lib, cu = L.lib(), torch.cuda.get_device_properties(0).multi_processor_count
+    k8, n8, at, odd = (k + 7) // 8 * 8, (n + 7) // 8 * 8, 256, 258   # addresses: nothing is read
+
+    def deep(cols, copies):
+        rounds = lambda t: -(-(-(-m // 256) * -(-cols // t)) // cu)  # noqa: E731
+        return (256 if 7 * rounds(256) <= 5 * rounds(128) else 128) if copies else 0
+    fwd = lib.crnn_linear_fwd_workspace(1, odd, k8, at, k8, m, n, k8)
+    bwd = lambda x, w, dx, dw: lib.crnn_linear_bwd_workspace(1, at, n8, x, k8, w, k8, 0, dx, dw, 0, m, n8, k8)  # noqa: E731
+    slabs = bwd(at, at, 0, 1)
+    splits = slabs // (n8 * k8 * 4)
+    return (deep(n, fwd), deep(k8, bwd(at, odd, 1, 0)), 256 if bwd(odd, at, 0, 1) > slabs else splits, splits)
+
+
+# rows, K, N and the plan on 256 CUs: tiles of the forward and of the input gradient (0: register-staged), of the weight gradient
+# (256, else its splits: 16 and 15 are those of 128 x 128 tiles, 64 x 64 ones would be cut into 4)
+DEEP = [((8192, 512, 1024), (128, 0, 16)),       # whole vectors
+        ((8190, 1024, 512), (0, 128, None)),
+        ((8195, 509, 1021), (256, 0, 15)),       # copies of x and w for the forward, nothing copied for dx and dw
+        ((25601, 261, 250), (128, 256, None)),   # copies throughout; 250 = 31 vectors and two columns
+        ((25605, 264, 264), (256, 256, None)),   # row and column remainders of whole vectors
+        ((32773, 1531, 765), (256, 256, 256)),   # copies of x, w and dy, remainders everywhere
+        ((32768, 768, 1536), (256, 256, 256))]
+
+
+@pytest.mark.parametrize("size,plan", DEEP)
+@pytest.mark.parametrize("kind,bias,res", [("none", None, False), ("gelu", "f32", False), ("silu", "same", True), ("relu", "f32", True),
+                                           ("none", "same", True)])
+def test_linear_of_large_batches(size, plan, kind, bias, res):
+    """the deep kernels with their own epilogue, the copies that they ask for, and the large tiles of the weight gradient; the plan
+    is asserted, so that another choice of tiles does not leave them without a test"""
+    m, k, n = size
+    got = linear_plan(m, k, n)
+    assert got[:2] == plan[:2] and plan[2] in (None, got[2]), got
+    dt = torch.bfloat16
+    g = gen(m + k + n)
+    x, w, dy = randn(g, m, k, dtype=dt), randn(g, n, k, dtype=dt, scale=1 / math.sqrt(k)), randn(g, m, n, dtype=dt)
+    b = randn(g, n, dtype=torch.float32 if bias == "f32" else dt) if bias else None
+    r = randn(g, m, n + 3, dtype=dt)[:, 2:2 + n] if res else None   # rows of odd pitch, 4 bytes off
+    leaves = [t.detach().requires_grad_(True) if t is not None else None for t in (x, w, b, r)]
+    y = crnn_hip.linear(leaves[0], leaves[1], leaves[2], activation=kind, residual=leaves[3])
+    grads = list(torch.autograd.grad(y, [t for t in leaves if t is not None], dy))
+    (ry, ey), (rx, ex), (rw, ew), (rb, eb) = linear_ref(x, w, b, r, dy, kind, dt)
+    within("y", y, ry, ey)
+    within("dx", grads[0], rx, ex)
+    within("dw", grads[1], rw, ew)
+    if b is not None:
+        within("db", grads[2], rb, eb + ET[b.dtype] * rb.abs())
+    if r is not None:
+        assert torch.equal(grads[-1], dy)
+    with torch.no_grad():
+        assert torch.equal(crnn_hip.linear(x, w, b, activation=kind, residual=r), y)
+    again = torch.autograd.grad(crnn_hip.linear(leaves[0], leaves[1], leaves[2], activation=kind, residual=leaves[3]),
+                                [t for t in leaves if t is not None], dy)
+    assert all(torch.equal(p, q) for p, q in zip(again, grads))   # no sum whose order changes
+
+
+def test_linear_keeps_what_lies_beside_its_rows():
+    """the deep kernels' outputs in wider buffers: y, z and dx fill their own columns and rows only"""
+    g = gen(91)
+    m, k, n, s = 25601, 264, 250, L.stream_ptr()
+    assert linear_plan(m, k, n)[:2] == (128, 256)
+    x, w, b, res, dy = (randn(g, *q, dtype=torch.bfloat16) for q in ((m, k), (n, k), (n,), (m, n), (m, n)))
+    y, z, dx = (torch.full((m + 3, c), 7.0, device=DEV, dtype=torch.bfloat16) for c in (n + 9, n + 6, k + 5))
+    need = L.lib().crnn_linear_fwd_workspace(1, x.data_ptr(), k, w.data_ptr(), k, m, n, k)
+    ws = torch.empty(max(need, 16), dtype=torch.uint8, device=DEV)
+    L.call("crnn_linear_fwd", 1, x.data_ptr(), k, w.data_ptr(), k, b.data_ptr(), 0, 2, res.data_ptr(), n, y.data_ptr(), n + 9, z.data_ptr(),
+           n + 6, ws.data_ptr(), need, m, n, k, s)
+    need = L.lib().crnn_linear_bwd_workspace(1, dy.data_ptr(), n, x.data_ptr(), k, w.data_ptr(), k, 2, 1, 0, 0, m, n, k)
+    ws = torch.empty(need, dtype=torch.uint8, device=DEV)
+    L.call("crnn_linear_bwd", 1, dy.data_ptr(), n, x.data_ptr(), k, w.data_ptr(), k, z.data_ptr(), n + 6, 2, dx.data_ptr(), k + 5, None, 0, None,
+           0, 0, ws.data_ptr(), need, m, n, k, s)
+    (ry, ey), (rx, ex), _, _ = linear_ref(x, w, b, res, dy, "gelu", torch.bfloat16)
+    rz = x.double() @ w.double().t().contiguous() + b.double()
+    ez = (k / 4 + 16) * U * (x.double().abs() @ w.double().abs().t().contiguous() + b.double().abs()) + ET[torch.bfloat16] * rz.abs()
+    for name, buf, c, ref, err in (("y", y, n, ry, ey), ("z", z, n, rz, ez), ("dx", dx, k, rx, ex)):
+        within(name, buf[:m, :c], ref, err)
+        assert (buf[m:] == 7.0).all() and (buf[:m, c:] == 7.0).all(), name
+
+
+@pytest.mark.parametrize("dt", TYPES)
+@pytest.mark.parametrize("off", [0, 1])
+def test_linear_in_launches_of_few_rows(dt, off):
+    """rows so far apart that a launch's 2 GiB hold 16 of them: 40 rows in launches of 16, 16 and 8, for x (forward and weight gradient),
+    then for dy (input and weight gradient), with the pointers of the residual, y and z moved along. off: a pitch that is not a
+    whole vector"""
+    es = 2 if dt == torch.bfloat16 else 4
+    ld = (1 << 27) // es - 8 + off
+    big = torch.empty(40 * ld, dtype=dt, device=DEV)
+    g = gen(92 + off)
+    m, k, n = 40, 72, 56
+    x, w, b = randn(g, m, k, dtype=dt), randn(g, n, k, dtype=dt, scale=0.2), randn(g, n)
+    res, dy = randn(g, m, n, dtype=dt), randn(g, m, n, dtype=dt)
+    far = big.as_strided((m, k), (ld, 1))
+    far.copy_(x)
+    leaves = [t.detach().requires_grad_(True) for t in (far, w, b, res)]
+    y = crnn_hip.linear(leaves[0], leaves[1], leaves[2], activation="silu", residual=leaves[3])
+    got = torch.autograd.grad(y, leaves, dy)
+    refs = linear_ref(x, w, b, res, dy, "silu", dt)
+    for name, a, (ref, err) in zip(("y", "dx", "dw", "db"), (y, got[0], got[1], got[2]), refs):
+        within(name, a, ref, err + (U if name == "db" else 0) * ref.abs())
+    fdy = big.as_strided((m, n), (ld, 1))
+    fdy.copy_(dy)
+    lx, lw = x.clone().requires_grad_(True), w.clone().requires_grad_(True)
+    got = torch.autograd.grad(crnn_hip.linear(lx, lw), (lx, lw), fdy)
+    refs = linear_ref(x, w, None, None, dy, "none", dt)
+    within("dx, far dy", got[0], *refs[1])
+    within("dw, far dy", got[1], *refs[2])
+    del big, far, fdy, leaves, y
+    torch.cuda.empty_cache()
+
+
+def test_linear_of_more_than_2_gib():
+    """x of more than 2 GiB: a launch of the deep kernel over the first 261888 rows and one of the rest"""
+    g = gen(93)
+    m, k, n = 262144 + 37, 4096, 128
+    x = torch.empty(m, k, device=DEV, dtype=torch.bfloat16)
+    for i in range(0, m, 65536):
+        x[i:i + 65536] = randn(g, min(65536, m - i), k, dtype=torch.bfloat16)
+    w, dy = randn(g, n, k, dtype=torch.bfloat16, scale=1 / 64), randn(g, m, n, dtype=torch.bfloat16)
+    assert linear_plan(m, k, n)[0] == 128
+    leaves = [t.detach().requires_grad_(True) for t in (x, w)]
+    y = crnn_hip.linear(*leaves, activation="gelu")
+    gx, gw = torch.autograd.grad(y, leaves, dy)
+    for lo, hi in ((0, 300), (261888 - 150, 261888 + 150), (m - 300, m)):   # where the launches begin, meet and end
+        (ry, ey), (rx, ex), _, _ = linear_ref(x[lo:hi], w, None, None, dy[lo:hi], "gelu", torch.bfloat16)
+        within(f"y {lo}", y[lo:hi], ry, ey)
+        within(f"dx {lo}", gx[lo:hi], rx, ex)
+    # the weight gradient over all rows, in parts: the references add, and so do the bounds (a split of the kernel's sum holds fewer rows
+    # than a part, and the parts' bounds on the rounding of their own results add up to no less than the whole's)
+    rw, ew = 0, 0
+    for i in range(0, m, 65536):
+        _, _, (r, e), _ = linear_ref(x[i:i + 65536], w, None, None, dy[i:i + 65536], "gelu", torch.bfloat16)
+        rw, ew = rw + r, ew + e
+    within("dw", gw, rw, ew)
+    del x, dy, y, gx, leaves
+    torch.cuda.empty_cache()
+
+
+@pytest.mark.parametrize("dt", TYPES)
+@pytest.mark.parametrize("m,n", [(65600, 40), (32800, 128), (16400, 250), (8200, 512), (8200, 1021), (2100, 2048), (2100, 4001), (2100, 8192),
+                                 (2100, 16384), (520, 16390)])
+def test_layer_norm_of_more_rows_than_a_grid(m, n, dt):
+    """each of the tiles with more rows than its forward's workgroups hold at once (2048 workgroups; wide rows: 512)"""
+    g = gen(m + n)
+    x, w, b, dy = randn(g, m, n, dtype=dt, shift=0.5), randn(g, n, shift=1.0, scale=0.3), randn(g, n), randn(g, m, n, dtype=dt)
+    leaves = [t.detach().requires_grad_(True) for t in (x, w, b)]
+    y = crnn_hip.layer_norm(*leaves)
+    got = [y] + list(torch.autograd.grad(y, leaves, dy))
+    for name, a, ref in zip(("y", "dx", "dw", "db"), got, ln_ref(x, w, b, dy, 1e-5, dt)):
+        within(name, a, *ref)
+
+
+@pytest.mark.parametrize("dt", TYPES)
+@pytest.mark.parametrize("direction", ["forward", "reverse", "both"])
+def test_gated_scan_of_many_sequences(direction, dt):
+    """1024 rows of channels or more: tiles of four waves, several of them, no segments"""
+    g = gen(95)
+    b, t, d = 1030, 53, 130
+    code = {"forward": 0, "reverse": 1, "both": 2}[direction]
+    lib = L.lib()
+    assert lib.crnn_gated_scan_workspace(L.dtype_code(dt), b, t, d, code) == 0
+    assert lib.crnn_gated_scan_ckpt_bytes(L.dtype_code(dt), b, t, d, code) == b * 4 * d * 4   # four tiles of 16 steps
+    f, v, h0 = randn(g, b, t, d, dtype=dt, scale=2.0, shift=1.0), randn(g, b, t, d, dtype=dt), randn(g, b, d)
+    scan_check(f, v, h0, None, direction, g, dt)
+    lens = torch.randint(0, t + 1, (b,), generator=g, device=DEV, dtype=torch.int32)
+    lens[:3] = torch.tensor([0, 1, t], device=DEV)
+    scan_check(f, v, None, lens, direction, g, dt)
+
+
+def test_gated_scan_held_steps():
+    """infinite logits hold the state: bf16 and fp32 gates are exactly 1 and 0 there, so the state moves only where it enters another
+    piece through the composed steps of the piece before. A wave holds 4 steps: of 10 .. 19 the pieces from 12 and from 16 are entered
+    that way. The first crossing composes steps 8 .. 11, two of which are not held: A a product of 2 gates that are not 1 (U), H a
+    sum of 2 products (4 U max|v|), one multiply-add (2 U), against the same steps walked one by one (the same again); the second composes
+    ones and zeros, exactly. Together 14 U max(|h|, |v|), and half a step of the type on each side"""
+    for dt in TYPES:
+        g = gen(96)
+        f, v, h0 = randn(g, 3, 45, 64, dtype=dt), randn(g, 3, 45, 64, dtype=dt), randn(g, 3, 64)
+        f[:, 10:20] = float("inf")
+        y = crnn_hip.gated_scan(f, v, h0=h0)
+        top = float(torch.maximum(v.abs().max().float(), h0.abs().max()))
+        held = y[:, 9:10].double().expand(3, 10, 64)
+        within("held", y[:, 10:20], held, 14 * U * top + 2 * ET[dt] * held.abs())
+        assert torch.equal(y[:, 12:13].expand(3, 8, 64), y[:, 12:20])   # one piece's state, and then the same through ones and zeros
