@@ -140,3 +140,50 @@ def test_dropout_seed_single_process_is_torch_seed():
     from crnn_hip.engine import dropout_seed
     assert dropout_seed(1234) == 1234
     assert dropout_seed(-1) == 0xFFFFFFFFFFFFFFFF
+
+
+def _glr_worker(rank, world, port, q):
+    os.environ.update(MASTER_ADDR="127.0.0.1", MASTER_PORT=str(port), RANK=str(rank), WORLD_SIZE=str(world), LOCAL_RANK=str(rank))
+    import sys
+    here = os.path.dirname(os.path.abspath(__file__))
+    sys.path.insert(0, os.path.join(here, "../rcnn-ocr_amd"))
+    from crnn_hip import dist as D
+    D.init_from_env("gloo")
+    try:
+        from crnn_hip.engine import CRNNEngine
+        from model.model import RCNN
+        ok = True
+        for decoder in ("ctc", "attn"):
+            offs = RCNN(num_classes=10, hidden_size=16, rnn_type="glr", decoder=decoder).flat_offsets()
+            n = sum(k for _, k in offs.values())
+            stages = ([["attn."]] if decoder == "attn" else []) + CRNNEngine.backward_stages()
+            for mb in (4, 4 << 20, 1 << 40):
+                g = torch.ones(n) * (rank + 1)
+                red = D.OverlappedAllReduce(g, offs, min_bucket_bytes=mb)
+                seen = set()
+                for st in stages:
+                    red.ready(st)
+                    seen |= {k for k in offs if k.startswith(tuple(st))}
+                    ok = ok and all(k in seen for lo, hi in red.issued for k, (s, c) in offs.items() if s < hi and s + c > lo)
+                red.finish()
+                spans = sorted(red.last_issued)
+                ok = ok and seen == set(offs) and spans[0][0] == 0 and spans[-1][1] == n
+                ok = ok and all(a[1] == b[0] for a, b in zip(spans, spans[1:])) and bool((g == world * (world + 1) // 2).all())
+        q.put((rank, ok))
+    finally:
+        dist.destroy_process_group()
+
+
+def test_overlapped_reduce_covers_the_gated_linear_recurrence_model():
+    """rnn_type="glr": its parameters lie in the flat buffer under the stages that the backward reports, with either head; every
+    bucket is issued once, after all it holds was reported"""
+    ctx = mp.get_context("spawn")
+    q = ctx.Queue()
+    port = _free_port()
+    ps = [ctx.Process(target=_glr_worker, args=(r, 2, port, q)) for r in range(2)]
+    for p in ps:
+        p.start()
+    res = [q.get(timeout=240) for _ in ps]
+    for p in ps:
+        p.join(timeout=60)
+    assert all(r[1] for r in res), res

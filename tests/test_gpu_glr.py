@@ -174,3 +174,140 @@ def test_surface_and_state_dict():
         RCNN(num_classes=40, rnn_type="gru")
     with pytest.raises(RuntimeError, match="HIP device"):
         m(torch.zeros(1, 3, 32, 64))
+
+
+# ------------------------------------------------------------------------------------------------ data parallel
+def _shard(rank):
+    from crnn_hip.recipe import synthetic_batch
+    x, _, tg, tl = synthetic_batch(8, 32, 128, 8, 40, seed=200 + rank)
+    return x.to(DEV), tg, tl
+
+
+def _flat_model(seed):
+    m = make(64, torch.bfloat16, seed=seed).to(DEV).train()
+    m.flatten_parameters_()
+    return m
+
+
+def _dp_worker(rank, world, port, q):
+    os.environ.update(MASTER_ADDR="127.0.0.1", MASTER_PORT=str(port), RANK=str(rank), WORLD_SIZE=str(world), LOCAL_RANK=str(rank),
+                      CRNN_SHARE_DEVICE="1", HSA_ENABLE_IPC_MODE_LEGACY="0")
+    import sys
+    here = os.path.dirname(os.path.abspath(__file__))
+    sys.path.insert(0, os.path.join(here, "../rcnn-ocr_amd"))
+    import torch.distributed as dist
+    try:
+        from crnn_hip import dist as D
+        from crnn_hip.engine import CRNNEngine
+        from crnn_hip.optim import FusedAdamW
+        D.init_from_env("gloo")
+        torch.cuda.set_device(0)
+        m = _flat_model(5 + rank)              # other weights on rank 1: the broadcast has to replace them
+        flat = m._flat_param.detach().cpu()    # (gloo: host tensors only)
+        D.broadcast_params(flat)
+        with torch.no_grad():
+            m._flat_param.copy_(flat)
+        m.mark_params_changed()
+        opt = FusedAdamW(m, lr=1e-3)
+        opt.zero_grad()
+        # the reducer as in deployment, on a host copy of the flat gradient that the hook fills with what each stage reports final
+        offs, host = m.flat_offsets(), torch.full_like(flat, float("nan"))
+        red = D.OverlappedAllReduce(host, offs, min_bucket_bytes=1 << 20)
+        stages = []
+
+        def hook(prefixes):
+            stages.append(list(prefixes))
+            for k, (s, n) in offs.items():
+                if k.startswith(tuple(prefixes)):
+                    host[s:s + n].copy_(m._flat_grad[s:s + n])
+            red.ready(prefixes)
+        m.stage_done = hook
+        x, tg, tl = _shard(rank)
+        ctc_loss(m(x), tg, tl).backward()
+        red.finish()
+        spans = sorted(red.last_issued)
+        tiled = len(spans) > 1 and spans[0][0] == 0 and spans[-1][1] == host.numel() and all(a[1] == b[0] for a, b in zip(spans, spans[1:]))
+        m._flat_grad.copy_(host)
+        opt.step(grad_scale=1.0 / world)
+        torch.cuda.synchronize()
+        q.put((rank, None, stages == CRNNEngine.backward_stages(), tiled, host.numpy(), m._flat_param.detach().cpu().numpy()))
+    except Exception:   # report to the parent instead of hanging it
+        import traceback
+        q.put((rank, traceback.format_exc(), False, False, None, None))
+    finally:
+        if dist.is_initialized():
+            dist.destroy_process_group()
+
+
+@pytest.mark.gpu
+def test_data_parallel_of_the_stack():
+    """two processes on the one GPU, a shard each: the stages report their gradients final in order, the buckets tile the flat
+    gradient, the reduced gradient is the sum of the shards' own, bit for bit, and both replicas take the same step as one process with
+    that sum"""
+    import socket
+
+    import torch.multiprocessing as mp
+
+    from crnn_hip.optim import FusedAdamW
+    with socket.socket() as s:
+        s.bind(("127.0.0.1", 0))
+        port = s.getsockname()[1]
+    ctx = mp.get_context("spawn")
+    q = ctx.Queue()
+    ps = [ctx.Process(target=_dp_worker, args=(r, 2, port, q)) for r in range(2)]
+    for p in ps:
+        p.start()
+    res = sorted((q.get(timeout=100) for _ in ps), key=lambda r: r[0])
+    for p in ps:
+        p.join(timeout=30)
+    for r in res:
+        assert r[1] is None, r[1]
+        assert r[2] and r[3]
+    m = _flat_model(5)
+    opt = FusedAdamW(m, lr=1e-3)
+    grads = []
+    for rank in range(2):
+        opt.zero_grad()
+        x, tg, tl = _shard(rank)
+        ctc_loss(m(x), tg, tl).backward()
+        grads.append(m._flat_grad.detach().clone())
+    m._flat_grad.copy_(grads[0] + grads[1])
+    for _, p in m.named_parameters():
+        assert p.grad is not None
+    opt.step(grad_scale=0.5)
+    want_g, want_p = (grads[0] + grads[1]).cpu(), m._flat_param.detach().cpu()
+    for r in res:
+        assert torch.equal(torch.from_numpy(r[4]), want_g)
+        assert torch.equal(torch.from_numpy(r[5]), want_p)
+
+
+@pytest.mark.gpu
+def test_stack_at_the_training_batch():
+    """256 lines of 32 frames at hidden 512, the batch at which the products run on their large tiles: output, input gradient and
+    parameter gradients against fp64, and a second backward that adds to the first's gradients in fp32. The bound of
+    test_stack_matches_fp64: 9 stored roundings per layer and direction in a chain, each at most 2^-8 of what it rounds"""
+    m = make(512, torch.bfloat16).to(DEV).train()
+    m.flatten_parameters_()
+    with torch.no_grad():
+        for k, v in m.named_parameters():
+            if k.startswith("enc_rnn.") and v.dim() == 2:
+                v.copy_(v.bfloat16().float())
+    eng = m._engine_for(torch.zeros(1, 3, 32, 8, device=DEV))
+    g = torch.Generator(device=DEV).manual_seed(12)
+    x, dout = (torch.randn(256, 32, 512, generator=g, device=DEV).bfloat16().float() for _ in range(2))
+    grads, _, _ = m._grad_views()
+    y, dx = eng.bilstm_stack(x, dout, grads)
+    p = {k: v.detach().double().requires_grad_(True) for k, v in m.named_parameters() if k.startswith("enc_rnn.")}
+    x64 = x.double().requires_grad_(True)
+    y64 = stack_fp64(x64, p, 2)
+    y64.backward(dout.double())
+    rel = lambda a, b: float((a.double() - b).norm() / b.norm())  # noqa: E731
+    assert rel(y, y64.detach()) < 7e-2 and rel(dx, x64.grad) < 7e-2
+    for k, v in p.items():
+        assert rel(grads[k], v.grad) < 7e-2, (k, rel(grads[k], v.grad))
+    first = {k: grads[k].clone() for k in p}
+    xs, ds = x.bfloat16(), dout.bfloat16()
+    _, saved = eng._rnn_forward(xs, 256, 32, True)
+    eng._rnn_backward(ds, saved, 256, 32, 1)
+    for k in p:
+        assert torch.equal(grads[k], first[k] + first[k]), k
