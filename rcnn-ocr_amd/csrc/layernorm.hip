@@ -285,36 +285,41 @@ __global__ __launch_bounds__(ln_threads<WPR>(), WPR == 1 ? 3 : 1) void ln_bwd_ke
   }
 }
 
+constexpr int kGridX = 1 << 20;   // most workgroups along the columns: 2^30 threads of the widest (a grid ends below 2^32)
+
 // out_w[n], out_b[n] (+)= the sum of G partial rows [G][2][N]: 64 columns of the 2N per workgroup, 16 row lanes, fixed order
 __global__ __launch_bounds__(1024) void ln_colsum_kernel(const float* __restrict__ part, int G, int N, float* __restrict__ dw,
                                                          float* __restrict__ db, int accumulate) {
   __shared__ float red[16][64];
   const int col = threadIdx.x & 63, rl = threadIdx.x >> 6;
-  const long j = (long)blockIdx.x * 64 + col;
   const long W = 2L * N;
-  float s = 0.f;
-  if (j < W) {
-    const float* p = part + j;
-    int g = rl;
-    for (; g + 7 * 16 < G; g += 8 * 16) {
-      float v[8];
+  for (long j0 = (long)blockIdx.x * 64; j0 < W; j0 += (long)gridDim.x * 64) {
+    const long j = j0 + col;
+    float s = 0.f;
+    if (j < W) {
+      const float* p = part + j;
+      int g = rl;
+      for (; g + 7 * 16 < G; g += 8 * 16) {
+        float v[8];
 #pragma unroll
-      for (int u = 0; u < 8; ++u) v[u] = p[(size_t)(g + 16 * u) * W];
+        for (int u = 0; u < 8; ++u) v[u] = p[(size_t)(g + 16 * u) * W];
 #pragma unroll
-      for (int u = 0; u < 8; ++u) s += v[u];
+        for (int u = 0; u < 8; ++u) s += v[u];
+      }
+      for (; g < G; g += 16) s += p[(size_t)g * W];
     }
-    for (; g < G; g += 16) s += p[(size_t)g * W];
-  }
-  red[rl][col] = s;
-  __syncthreads();
-  if (rl == 0 && j < W) {
+    red[rl][col] = s;
+    __syncthreads();
+    if (rl == 0 && j < W) {
 #pragma unroll
-    for (int r = 1; r < 16; ++r) s += red[r][col];
-    float* o = j < N ? dw : db;
-    if (o) {
-      const long n = j < N ? j : j - N;
-      o[n] = accumulate ? o[n] + s : s;
+      for (int r = 1; r < 16; ++r) s += red[r][col];
+      float* o = j < N ? dw : db;
+      if (o) {
+        const long n = j < N ? j : j - N;
+        o[n] = accumulate ? o[n] + s : s;
+      }
     }
+    __syncthreads();   // red is the next columns'
   }
 }
 
@@ -336,6 +341,19 @@ __device__ __forceinline__ void block_sum2(float& a, float& b, float (*red)[32],
   }
 }
 
+// f(n, p, q) adds column n's terms of two sums; 64 columns of a lane at a time, so that the longest rows (2^30) add 2^14 sums of 64
+// terms instead of 2^20 terms one by one
+template <class F> __device__ __forceinline__ void wide_sum2(int N, float& a, float& b, F f) {
+  a = b = 0.f;
+  for (int n0 = threadIdx.x; n0 < N; n0 += 64 * LW) {
+    float p = 0.f, q = 0.f;
+    const int end = min(N, n0 + 64 * LW);
+    for (int n = n0; n < end; n += LW) f(n, p, q);
+    a += p;
+    b += q;
+  }
+}
+
 template <typename T>
 __global__ __launch_bounds__(LW) void ln_fwd_wide_kernel(const T* __restrict__ x, long ldx, const float* __restrict__ w,
                                                          const float* __restrict__ b, T* __restrict__ y, long ldy,
@@ -345,16 +363,16 @@ __global__ __launch_bounds__(LW) void ln_fwd_wide_kernel(const T* __restrict__ x
   const float inv = 1.f / (float)N;
   for (long m = blockIdx.x; m < M; m += gridDim.x) {
     const T* row = x + m * ldx;
-    float s = 0.f, z = 0.f;
-    for (int n = threadIdx.x; n < N; n += LW) s += tof(row[n]);
+    float s, z;
+    wide_sum2(N, s, z, [&](int n, float& p, float&) { p += tof(row[n]); });
     block_sum2(s, z, red, 0);
     const float m0 = s * inv;
-    float d = 0.f, q = 0.f;
-    for (int n = threadIdx.x; n < N; n += LW) {
+    float d, q;
+    wide_sum2(N, d, q, [&](int n, float& p, float& r) {
       const float e = tof(row[n]) - m0;
-      d += e;
-      q += e * e;
-    }
+      p += e;
+      r += e * e;
+    });
     block_sum2(d, q, red, 1);
     d *= inv;
     const float mu = m0 + d, rs = 1.f / sqrtf(fmaxf(q * inv - d * d, 0.f) + eps);
@@ -377,12 +395,12 @@ __global__ __launch_bounds__(LW) void ln_bwd_wide_kernel(const T* __restrict__ d
   int set = 0;
   for (long m = blockIdx.x; m < M; m += gridDim.x) {
     const float mu = mean[m], rs = rstd[m];
-    float s1 = 0.f, s2 = 0.f;
-    for (int n = threadIdx.x; n < N; n += LW) {
+    float s1, s2;
+    wide_sum2(N, s1, s2, [&](int n, float& p, float& q) {
       const float g = tof(dy[m * lddy + n]) * (w ? w[n] : 1.f);
-      s1 += g;
-      s2 += g * (tof(x[m * ldx + n]) - mu) * rs;
-    }
+      p += g;
+      q += g * (tof(x[m * ldx + n]) - mu) * rs;
+    });
     block_sum2(s1, s2, red, set);
     set ^= 1;
     s1 *= inv;
@@ -402,26 +420,29 @@ __global__ __launch_bounds__(256) void ln_wgrad_wide_kernel(const T* __restrict_
                                                             const float* __restrict__ mean, const float* __restrict__ rstd,
                                                             float* __restrict__ part, long M, int N, int G) {
   __shared__ float red[2][4][64];
-  const int col = threadIdx.x & 63, rl = threadIdx.x >> 6;
-  const int n = blockIdx.x * 64 + col, g = blockIdx.y;
-  float sw = 0.f, sb = 0.f;
-  if (n < N)
-    for (long m = (long)g * 4 + rl; m < M; m += 4L * G) {
-      const float d = tof(dy[m * lddy + n]);
-      sb += d;
-      sw += d * (tof(x[m * ldx + n]) - mean[m]) * rstd[m];
-    }
-  red[0][rl][col] = sw;
-  red[1][rl][col] = sb;
-  __syncthreads();
-  if (rl == 0 && n < N) {
+  const int col = threadIdx.x & 63, rl = threadIdx.x >> 6, g = blockIdx.y;
+  for (long n0 = (long)blockIdx.x * 64; n0 < N; n0 += (long)gridDim.x * 64) {
+    const long n = n0 + col;
+    float sw = 0.f, sb = 0.f;
+    if (n < N)
+      for (long m = (long)g * 4 + rl; m < M; m += 4L * G) {
+        const float d = tof(dy[m * lddy + n]);
+        sb += d;
+        sw += d * (tof(x[m * ldx + n]) - mean[m]) * rstd[m];
+      }
+    red[0][rl][col] = sw;
+    red[1][rl][col] = sb;
+    __syncthreads();
+    if (rl == 0 && n < N) {
 #pragma unroll
-    for (int r = 1; r < 4; ++r) {
-      sw += red[0][r][col];
-      sb += red[1][r][col];
+      for (int r = 1; r < 4; ++r) {
+        sw += red[0][r][col];
+        sb += red[1][r][col];
+      }
+      part[(size_t)g * 2 * N + n] = sw;
+      part[(size_t)g * 2 * N + N + n] = sb;
     }
-    part[(size_t)g * 2 * N + n] = sw;
-    part[(size_t)g * 2 * N + N + n] = sb;
+    __syncthreads();   // red is the next columns'
   }
 }
 
@@ -513,8 +534,8 @@ int ln_bwd_t(const void* dy, long lddy, const void* x, long ldx, const float* w,
   } else if (M > 0) {
     if (part) {   // before dx: dx may be dres, and neither dy nor x may be dx, so the order is free; kept first
       G = ln_wide_slices(M);
-      hipLaunchKernelGGL(ln_wgrad_wide_kernel<T>, dim3((N + 63) / 64, G), dim3(256), 0, st, (const T*)dy, lddy, (const T*)x, ldx,
-                         mean, rstd, part, M, N, G);
+      hipLaunchKernelGGL(ln_wgrad_wide_kernel<T>, dim3(grid_for(N, 64, kGridX), G), dim3(256), 0, st, (const T*)dy, lddy, (const T*)x,
+                         ldx, mean, rstd, part, M, N, G);
       rc = (int)hipGetLastError();
     }
     if (!rc && dx) {
@@ -525,7 +546,7 @@ int ln_bwd_t(const void* dy, long lddy, const void* x, long ldx, const float* w,
     }
   }
   if (rc || !part) return rc;
-  hipLaunchKernelGGL(ln_colsum_kernel, dim3((int)((2L * N + 63) / 64)), dim3(1024), 0, st, part, G, N, dw, db, accumulate);
+  hipLaunchKernelGGL(ln_colsum_kernel, dim3(grid_for(2L * N, 64, kGridX)), dim3(1024), 0, st, part, G, N, dw, db, accumulate);
   return (int)hipGetLastError();
 }
 

@@ -1059,3 +1059,42 @@ def test_gated_scan_held_steps():
         held = y[:, 9:10].double().expand(3, 10, 64)
         within("held", y[:, 10:20], held, 14 * U * top + 2 * ET[dt] * held.abs())
         assert torch.equal(y[:, 12:13].expand(3, 8, 64), y[:, 12:20])   # one piece's state, and then the same through ones and zeros
+
+
+@pytest.mark.parametrize("dt", TYPES)
+def test_layer_norm_of_very_wide_rows(dt):
+    """a weight gradient over more than 2^27 columns (whose sums in one lane a column of 16 rows would be a grid of 2^32 threads), and the
+    statistics of such rows: a lane adds 64 terms at a time and then 2048 of those sums, the workgroup its 1024 lanes, so a sum of n terms is off by
+    less than (64 + n / 65536 + 16) U of their magnitudes"""
+    g = gen(98)
+    m, n = 2, (1 << 27) + 69
+    K = (64 + n / 65536 + 64) * U
+    x, dy = (torch.empty(m, n, device=DEV, dtype=dt) for _ in range(2))
+    for t in (x, dy):
+        for i in range(m):
+            t[i] = randn(g, n, dtype=dt, shift=0.5)
+    w, b = randn(g, n, shift=1.0, scale=0.3), randn(g, n)
+    leaves = [t.detach().requires_grad_(True) for t in (x, w, b)]
+    y = crnn_hip.layer_norm(*leaves)
+    gx, gw, gb = torch.autograd.grad(y, leaves, dy)
+    y = y.detach()
+    # the reference piece by piece of the columns, its sums first
+    cols = [slice(i, min(n, i + (1 << 25))) for i in range(0, n, 1 << 25)]
+    d = lambda t, c: t[..., c].detach().double()  # noqa: E731
+    mean = sum(d(x, c).sum(1, keepdim=True) for c in cols) / n
+    rs = 1 / (sum(((d(x, c) - mean) ** 2).sum(1, keepdim=True) for c in cols) / n + 1e-5).sqrt()
+    s1, s2, a1, a2 = (sum(f(d(dy, c) * d(w, c), (d(x, c) - mean) * rs).sum(1, keepdim=True) for c in cols) / n
+                      for f in (lambda p, q: p, lambda p, q: p * q, lambda p, q: p.abs(), lambda p, q: (p * q).abs()))
+    for c in cols:
+        xh, dyc, wc = (d(x, c) - mean) * rs, d(dy, c), d(w, c)
+        R = 1 + rs * d(x, c).abs().max()
+        exh = K * (xh.abs() + R)
+        ref = xh * wc + d(b, c)
+        within("y", y[:, c], ref, ET[dt] * ref.abs() + exh * wc.abs() + K * (ref.abs() + d(b, c).abs()))
+        gg = dyc * wc
+        ref = rs * (gg - s1 - xh * s2)
+        within("dx", gx[:, c], ref, ET[dt] * ref.abs() + rs * K * (gg.abs() + a1 + xh.abs() * a2 + R * (s2.abs() + xh.abs() * a1)))
+        within("dw", gw[c], (dyc * xh).sum(0), (dyc.abs() * exh).sum(0) + 8 * U * (dyc * xh).abs().sum(0))
+        within("db", gb[c], dyc.sum(0), 8 * U * dyc.abs().sum(0))
+    del x, dy, y, gx, gw, gb, leaves
+    torch.cuda.empty_cache()
