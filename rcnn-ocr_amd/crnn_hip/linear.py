@@ -22,7 +22,8 @@ def linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] =
     read as they lie, except that the largest bf16 products copy rows that are not 16-byte aligned multiples of 8 elements into
     such ones first. weight, and each row of x, stays under 2 GiB. Runs on x's device and its current torch stream; capturable
     (a captured backward is refused while an eager graph of its leaves, built on the default stream, is alive). ValueError for
-    arguments that do not fit, RuntimeError for CPU tensors."""
+    arguments that do not fit, RuntimeError for CPU
+    tensors and where it is traced (torch.compile, make_fx: torch.compiler.disable keeps it out) or differentiated by torch.func."""
     global _op
     if _op is None:
         _op = L.ops().linear.default

@@ -17,7 +17,8 @@ def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Opt
     gradients are fp32, y is rounded once to x's dtype. Differentiable once in x, weight and bias; the weight gradients
     add the rows in a fixed order. Runs on x's device and its current torch stream; capturable (a captured backward is
     refused while an eager graph of its leaves, built on the default stream, is alive). ValueError for arguments that do not
-    fit, RuntimeError for CPU tensors."""
+    fit, RuntimeError for CPU
+    tensors and where it is traced (torch.compile, make_fx: torch.compiler.disable keeps it out) or differentiated by torch.func."""
     global _op
     if _op is None:
         _op = L.ops().layer_norm.default

@@ -7,6 +7,7 @@
 // of the tensors' device and calls it. Its symbols are those of the libcrnn_hip.so that crnn_hip/_lib.py has loaded.
 #include <ATen/ATen.h>
 #include <c10/core/DeviceGuard.h>
+#include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <c10/hip/HIPGraphsC10Utils.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/autograd/custom_function.h>
@@ -30,7 +31,7 @@ int dtype_code(const char* op, const Tensor& t) {
   return CRNN_F32;
 }
 void require_device(const Tensor& t) {
-  TORCH_CHECK(t.is_cuda(), "crnn_hip ops run only on a HIP device (no CPU fallback); got a CPU tensor");
+  TORCH_CHECK(t.is_cuda(), "crnn_hip ops run only on a HIP device (no CPU fallback); got a tensor on ", t.device());
 }
 void check(const char* op, const char* name, const Tensor& t, at::IntArrayRef shape, const Tensor& like) {
   TORCH_CHECK_VALUE(t.sizes() == shape, op, ": ", name, " must have shape ", shape, ", got ", t.sizes());
@@ -41,6 +42,22 @@ void check_type(const char* op, const char* name, const Tensor& t, at::ScalarTyp
                     t.scalar_type());
 }
 bool has(const OptTensor& t) { return t.has_value() && t->defined(); }
+// The kernels take addresses, so only plain tensors, run at once, will do. Tracers (torch.compile, make_fx, fake tensors), torch.func's
+// derivatives and subclasses with a __torch_dispatch__ are refused: make_fx over real tensors would record the results' allocation and not
+// the kernel that fills them. (torch.vmap calls the operator for each sample on plain tensors.)
+void check_eager(const char* op, std::initializer_list<OptTensor> ts) {
+  using c10::DispatchKey;
+  using Mode = c10::impl::TorchDispatchModeTLS;
+  using Key = c10::impl::TorchDispatchModeKey;
+  static constexpr c10::DispatchKeySet wrapped(
+      {DispatchKey::Python, DispatchKey::FuncTorchGradWrapper, DispatchKey::FuncTorchBatched, DispatchKey::Functionalize, DispatchKey::Batched});
+  bool plain = true;
+  for (const OptTensor& t : ts) plain = plain && !(has(t) && t->unsafeGetTensorImpl()->key_set().has_any(wrapped));
+  if (Mode::any_modes_set())
+    plain = plain && !Mode::get_mode(Key::FAKE) && !Mode::get_mode(Key::PROXY) && !Mode::get_mode(Key::FUNCTIONAL);
+  TORCH_CHECK(plain, op, " runs eagerly, on plain tensors: no tracing (torch.compile, make_fx, fake tensors), no torch.func derivatives, no "
+              "subclasses with a __torch_dispatch__; torch.compiler.disable keeps it out of a compiled region");
+}
 // whether autograd has to record the call. Forward-mode tangents are refused: a plain call would drop them silently
 bool records(const char* op, std::initializer_list<OptTensor> ts) {
   bool grad = false;
@@ -210,6 +227,7 @@ Tensor layer_norm(const Tensor& x, const OptTensor& weight, const OptTensor& bia
     check_type("layer_norm", i ? "bias" : "weight", *p, at::kFloat, at::kFloat);
   }
   TORCH_CHECK_VALUE(eps >= 0, "layer_norm: eps must be >= 0, got ", eps);
+  check_eager("layer_norm", {x, weight, bias});
   require_device(x);
   const c10::OptionalDeviceGuard guard(x.device());
   if (records("layer_norm", {x, weight, bias}))
@@ -302,6 +320,7 @@ Tensor linear(const Tensor& x, const Tensor& weight, const OptTensor& bias, int6
     check("linear", "residual", *residual, shape, x);
     check_type("linear", "residual", *residual, x.scalar_type(), x.scalar_type());
   }
+  check_eager("linear", {x, weight, bias, residual});
   require_device(x);
   const c10::OptionalDeviceGuard guard(x.device());
   if (records("linear", {x, weight, bias, residual}))
@@ -399,6 +418,7 @@ std::tuple<Tensor, Tensor> gated_scan(const Tensor& f, const Tensor& v, const Op
   if (has(lengths))
     TORCH_CHECK_VALUE(lengths->dim() == 1 && lengths->size(0) == B && (lengths->scalar_type() == at::kInt || lengths->scalar_type() == at::kLong),
                       "gated_scan: lengths must be an int32 or int64 tensor of shape [", B, "], got ", lengths->scalar_type(), " ", lengths->sizes());
+  check_eager("gated_scan", {f, v, h0, lengths});
   require_device(f);
   const c10::OptionalDeviceGuard guard(f.device());
   OptTensor len;
@@ -418,6 +438,7 @@ std::tuple<Tensor, Tensor> gated_scan_step(const Tensor& f, const Tensor& v, con
   check_scan(op, f, v, 2);
   check(op, "state", state, f.sizes(), f);
   check_type(op, "state", state, at::kFloat, at::kFloat);
+  check_eager(op, {f, v, state, out_state});
   TORCH_CHECK(!records(op, {f, v, state, out_state}),
               "gated_scan_step is inference only: use gated_scan(..., return_state=True) where gradients are needed");
   if (has(out_state)) {

@@ -197,3 +197,32 @@ def test_c_gated_scan_refusals():
         assert lib.crnn_gated_scan_fwd(1, None, 0, 0, None, 0, 0, None, None, None, 0, 0, None, None, None, 0, b, t, d, 0, None) == 0
     _refused("crnn_gated_scan_bwd", 1, P, 64, 64, P, 64, 64, P, 64, 64, None, None, None, P, 64, 64, P, 64, 64, None, None, 0, 1, 1,
              64, 0, None, match="null")
+
+
+def _operators(x):
+    """the four entry points on one [4, 6] input"""
+    return {"layer_norm": lambda: crnn_hip.layer_norm(x), "linear": lambda: crnn_hip.linear(x, torch.zeros(3, 6)),
+            "gated_scan": lambda: crnn_hip.gated_scan(x[None], x[None]), "gated_scan_step": lambda: crnn_hip.gated_scan_step(x, x, x)[0]}
+
+
+@pytest.mark.parametrize("op", ["layer_norm", "linear", "gated_scan", "gated_scan_step"])
+def test_tracing_and_transforms_are_refused(op):
+    """they run eagerly on plain tensors: a trace would hold the results' allocation and not the kernel that fills them"""
+    from torch._subclasses.fake_tensor import FakeTensorMode
+    from torch.fx.experimental.proxy_tensor import make_fx
+    from torch.utils._python_dispatch import TorchDispatchMode
+    with FakeTensorMode(), pytest.raises(RuntimeError, match=f"{op} runs eagerly"):
+        _operators(torch.zeros(4, 6))[op]()
+    for mode in ("real", "fake", "symbolic"):
+        with pytest.raises(RuntimeError, match=f"{op} runs eagerly"):
+            make_fx(lambda x: _operators(x)[op](), tracing_mode=mode)(X)
+    with pytest.raises(RuntimeError, match=f"{op} runs eagerly"):
+        torch.func.grad(lambda x: _operators(x)[op]().sum())(X)
+    with pytest.raises(Exception, match=f"{op} runs eagerly"):
+        torch.compile(lambda x: _operators(x)[op]() + 1, backend="eager")(X)
+
+    class Count(TorchDispatchMode):   # a mode that only watches does not stand in the way: the call gets as far as the device
+        def __torch_dispatch__(self, func, types, args=(), kwargs=None):
+            return func(*args, **(kwargs or {}))
+    with Count(), pytest.raises(RuntimeError, match="HIP device"):
+        _operators(X)[op]()

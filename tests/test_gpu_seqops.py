@@ -1098,3 +1098,14 @@ def test_layer_norm_of_very_wide_rows(dt):
         within("db", gb[c], dyc.sum(0), 8 * U * dyc.abs().sum(0))
     del x, dy, y, gx, gw, gb, leaves
     torch.cuda.empty_cache()
+
+
+def test_beside_a_compiled_region_and_under_vmap():
+    """torch.compiler.disable keeps an operator out of a compiled function; vmap calls it for each sample"""
+    g = gen(99)
+    x, w = randn(g, 5, 7, 16), randn(g, 24, 16)
+    op = torch.compiler.disable(lambda x: crnn_hip.linear(crnn_hip.layer_norm(x), w))
+    want = torch.relu(crnn_hip.linear(crnn_hip.layer_norm(2 * x), w))
+    assert torch.equal(torch.compile(lambda x: torch.relu(op(2 * x)), backend="eager")(x), want)
+    assert torch.equal(torch.vmap(lambda t: crnn_hip.layer_norm(t))(x), crnn_hip.layer_norm(x))
+    assert torch.equal(torch.vmap(lambda t: crnn_hip.gated_scan(t[None], t[None])[0])(x), crnn_hip.gated_scan(x, x))
