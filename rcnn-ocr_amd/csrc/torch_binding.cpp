@@ -68,7 +68,9 @@ bool records(const char* op, std::initializer_list<OptTensor> ts) {
   }
   return grad && at::GradMode::is_enabled();
 }
-Tensor contiguous(const OptTensor& t) { return has(t) ? t->contiguous() : Tensor(); }
+// the values where the memory holds their negatives (views such as z.conj().imag, also as upstream gradients)
+Tensor values(const Tensor& t) { return t.is_neg() ? t.resolve_neg() : t; }
+Tensor contiguous(const OptTensor& t) { return has(t) ? values(*t).contiguous() : Tensor(); }
 void* ptr(const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
 float* fptr(const Tensor& t) { return (float*)ptr(t); }
 
@@ -77,7 +79,8 @@ struct Rows {
   Tensor t;
   int64_t m, ld;
 };
-Rows rows(const Tensor& t) {
+Rows rows(const Tensor& t_) {
+  const Tensor t = values(t_);
   const int64_t n = t.size(-1), m = n ? t.numel() / n : 0, d = t.dim();
   if (t.is_contiguous()) return {t, m, n};
   if (d >= 2 && (t.stride(-1) == 1 || n == 1) && t.stride(-2) >= n) {
@@ -88,7 +91,7 @@ Rows rows(const Tensor& t) {
   return {t.contiguous(), m, n};
 }
 // channels contiguous
-Tensor chan(const Tensor& t) { return t.stride(-1) == 1 || t.size(-1) == 1 ? t : t.contiguous(); }
+Tensor chan(const Tensor& t) { return t.stride(-1) == 1 || t.size(-1) == 1 ? values(t) : t.contiguous(); }
 
 Tensor bytes(size_t n, const Tensor& like) {
   return n ? at::empty({(int64_t)n}, like.options().dtype(at::kByte)) : Tensor();
@@ -198,7 +201,7 @@ struct LayerNormFn : public torch::autograd::Function<LayerNormFn> {
       const c10::OptionalDeviceGuard guard(x.device());
       check_capture("layer_norm");
       const Rows xr = rows(x), dy = rows(g[0]);
-      const Tensor w = contiguous(kept[1]), stats = kept[2].contiguous();
+      const Tensor w = contiguous(kept[1]), stats = contiguous(kept[2]);
       const int64_t n = x.size(-1), m = stats.numel() / 2;
       const int dt = dtype_code("layer_norm", x);
       if (need_x) out[0] = at::empty(x.sizes(), x.options());
@@ -366,11 +369,11 @@ struct GatedScanFn : public torch::autograd::Function<GatedScanFn> {
       at::AutoDispatchBelowADInplaceOrView below;
       const c10::OptionalDeviceGuard guard(kept[0].device());
       check_capture("gated_scan");
-      const Tensor f = chan(kept[0]), v = chan(kept[1]), len = contiguous(kept[2]), ckpt = kept[3].contiguous();
+      const Tensor f = chan(kept[0]), v = chan(kept[1]), len = contiguous(kept[2]), ckpt = contiguous(kept[3]);
       const int dt = dtype_code("gated_scan", f);
       // only the final state was used: no upstream gradient for y
       const Tensor dy = g[0].defined() ? chan(g[0]) : at::zeros(f.sizes(), f.options());
-      const Tensor dhT = g.size() > 1 && g[1].defined() ? g[1].contiguous() : Tensor();
+      const Tensor dhT = g.size() > 1 && g[1].defined() ? contiguous(g[1]) : Tensor();
       const auto opt = f.options().memory_format(at::MemoryFormat::Contiguous);
       Tensor df = at::empty(f.sizes(), opt), dv = at::empty(f.sizes(), opt), dh0 = need_h ? floats({B, D}, f) : Tensor();
       const size_t need = crnn_gated_scan_workspace(dt, B, T, D, dir);
@@ -444,7 +447,7 @@ std::tuple<Tensor, Tensor> gated_scan_step(const Tensor& f, const Tensor& v, con
   if (has(out_state)) {
     check(op, "out_state", *out_state, f.sizes(), f);
     check_type(op, "out_state", *out_state, at::kFloat, at::kFloat);
-    TORCH_CHECK_VALUE(out_state->is_contiguous(), op, ": out_state must be contiguous");
+    TORCH_CHECK_VALUE(out_state->is_contiguous() && !out_state->is_neg(), op, ": out_state must be contiguous, and no negated view");
     TORCH_CHECK_VALUE((out_state->data_ptr() == state.data_ptr() && state.is_contiguous()) || apart(*out_state, state), op,
                       ": out_state overlaps state without being it");
     TORCH_CHECK_VALUE(apart(*out_state, f) && apart(*out_state, v), op, ": out_state overlaps f or v");
@@ -453,7 +456,7 @@ std::tuple<Tensor, Tensor> gated_scan_step(const Tensor& f, const Tensor& v, con
   const c10::OptionalDeviceGuard guard(f.device());
   if (has(out_state)) torch::autograd::impl::bump_version(*out_state);   // a graph that saved it has to notice
   Tensor out = has(out_state) ? *out_state : floats(f.sizes(), f);
-  Tensor y = scan_run(chan(f.unsqueeze(1)), chan(v.unsqueeze(1)), state.contiguous(), Tensor(), 0, out, Tensor());
+  Tensor y = scan_run(chan(f.unsqueeze(1)), chan(v.unsqueeze(1)), contiguous(state), Tensor(), 0, out, Tensor());
   return {y.squeeze(1), out};
 }
 

@@ -226,3 +226,8 @@ def test_tracing_and_transforms_are_refused(op):
             return func(*args, **(kwargs or {}))
     with Count(), pytest.raises(RuntimeError, match="HIP device"):
         _operators(X)[op]()
+
+
+def test_step_refuses_a_negated_output():
+    with pytest.raises(ValueError, match="negated"):
+        crnn_hip.gated_scan_step(X, X, X, out_state=torch._neg_view(torch.zeros(4, 6)))

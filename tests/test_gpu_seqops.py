@@ -1109,3 +1109,26 @@ def test_beside_a_compiled_region_and_under_vmap():
     assert torch.equal(torch.compile(lambda x: torch.relu(op(2 * x)), backend="eager")(x), want)
     assert torch.equal(torch.vmap(lambda t: crnn_hip.layer_norm(t))(x), crnn_hip.layer_norm(x))
     assert torch.equal(torch.vmap(lambda t: crnn_hip.gated_scan(t[None], t[None])[0])(x), crnn_hip.gated_scan(x, x))
+
+
+def test_negated_views():
+    """tensors whose memory holds the values' negatives (z.conj().imag): the values count, in inputs and upstream gradients"""
+    g = gen(100)
+    neg = lambda *s: torch._neg_view(randn(g, *s))  # noqa: E731   (in any layout; z.conj().imag has rows of pairs)
+    thin = torch.complex(randn(g, 6, 1), randn(g, 6, 1)).conj().imag
+    assert thin.is_neg()
+    x, w, f, h, st = neg(6, 16), neg(8, 16), neg(2, 5, 16), neg(2, 16), neg(6, 16)
+    for fn, args in ((crnn_hip.layer_norm, (x, w[0], w[1])), (lambda x, w, b, r: crnn_hip.linear(x, w, b, residual=r), (x, w, w[:, 0], neg(6, 8))),
+                     (crnn_hip.linear, (thin, neg(8, 1))), (lambda f, h: crnn_hip.gated_scan(f, f, h0=h), (f, h)),
+                     (lambda x, s: torch.cat(crnn_hip.gated_scan_step(x, x, s)), (x, st))):
+        assert any(a.is_neg() for a in args)
+        want = fn(*[a.clone() for a in args])
+        assert not any(a.clone().is_neg() for a in args)
+        assert torch.equal(fn(*args), want)
+    for fn, args in ((crnn_hip.layer_norm, (x,)), (crnn_hip.linear, (x, w)), (crnn_hip.gated_scan, (f, f))):
+        leaves = [a.clone().requires_grad_(True) for a in args]
+        y = fn(*leaves)
+        dy = neg(*y.shape)
+        got = torch.autograd.grad(y, leaves, dy, retain_graph=True)
+        for a, b in zip(got, torch.autograd.grad(y, leaves, dy.clone())):
+            assert torch.equal(a, b)
