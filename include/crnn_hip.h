@@ -600,15 +600,16 @@ int crnn_linear_bwd(int dtype, const void* dy, long lddy, const void* x, long ld
  * [0, D/2) forward and [D/2, D) backward in time (D even; the bidirectional encoder's [forward | reverse] rows). T, D <= 2^30.
  * lengths (NULL: all T) int32 [B], clamped to [0, T]: steps t >= lengths[b] are not read and get y = 0.
  * h0 (NULL: 0) fp32 [B][D]: the state before the first step; hT (NULL: not stored) fp32 [B][D]: the one after the last
- * (h0 where the length is 0; hT may be h0 where the workspace is 0, e.g. for T <= 8). ckpt (NULL: inference): crnn_gated_scan_ckpt_bytes, fp32 states that the
- * backward recomputes h from. ws: crnn_gated_scan_workspace bytes (the segment summaries of long, few sequences). */
+ * (h0 where the length is 0; hT may be h0 where the workspace is 0, e.g. for T <= 8). ckpt (NULL: inference):
+ * crnn_gated_scan_ckpt_bytes, fp32 states that the backward recomputes h from. ws: crnn_gated_scan_workspace bytes (the segment summaries of long, few sequences). */
 size_t crnn_gated_scan_ckpt_bytes(int dtype, int B, int T, int D, int dir);
 size_t crnn_gated_scan_workspace(int dtype, int B, int T, int D, int dir);
 int crnn_gated_scan_fwd(int dtype, const void* f, long fsb, long fst, const void* v, long vsb, long vst, const float* h0,
                         const int* lengths, void* y, long ysb, long yst, float* hT, float* ckpt, float* ws,
                         size_t ws_bytes, int B, int T, int D, int dir, void* stream);
 /* G_t = dy_t + a_{t+1} G_{t+1} (+ dhT at the last step); df_t = G_t (h_{t-1} - v_t) a_t (1 - a_t), dv_t = G_t (1 - a_t),
- * dh0 = a_first G_first; zero at t >= lengths[b]. dhT (NULL: 0), dh0 (NULL: not stored) fp32 [B][D]. */
+ * dh0 = a_first G_first; zero at t >= lengths[b]. dhT (NULL: 0), dh0 (NULL: not stored) fp32 [B][D]; dh0 may be dhT where the
+ * workspace is 0. */
 int crnn_gated_scan_bwd(int dtype, const void* dy, long dsb, long dst, const void* f, long fsb, long fst, const void* v,
                         long vsb, long vst, const int* lengths, const float* dhT, const float* ckpt, void* df, long gsb,
                         long gst, void* dv, long wsb, long wst, float* dh0, float* ws, size_t ws_bytes, int B, int T,

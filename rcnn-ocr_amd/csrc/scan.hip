@@ -647,6 +647,8 @@ int crnn_gated_scan_bwd(int dtype, const void* dy, long dsb, long dst, const voi
   if (!dy || !f || !v || !df || !dv || !ckpt) return crnn_set_error(hipErrorInvalidValue, "gated_scan_bwd: null dy / f / v / df / dv / ckpt");
   const size_t need = crnn_gated_scan_workspace(dtype, B, T, D, dir);
   if (need && (!ws || ws_bytes < need)) return crnn_set_error(hipErrorInvalidValue, "gated_scan_bwd: workspace too small");
+  if (need && dh0 && dh0 == dhT)   // the first segment's workgroup would overwrite what the others still read
+    return crnn_set_error(hipErrorInvalidValue, "gated_scan_bwd: dh0 == dhT needs an unsegmented sequence (workspace 0)");
   ScanArgs a = {};
   a.dy = dy; a.dsb = dsb; a.dst = dst;
   a.f = f; a.fsb = fsb; a.fst = fst;

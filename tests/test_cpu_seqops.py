@@ -231,3 +231,16 @@ def test_tracing_and_transforms_are_refused(op):
 def test_step_refuses_a_negated_output():
     with pytest.raises(ValueError, match="negated"):
         crnn_hip.gated_scan_step(X, X, X, out_state=torch._neg_view(torch.zeros(4, 6)))
+
+
+def test_c_gated_scan_bwd_refuses_a_state_gradient_over_its_input():
+    """segments run at once: the first one's dh0 may not be written over the dhT that the others still read"""
+    lib = L.lib()
+    seg = lib.crnn_gated_scan_workspace(1, 1, 16384, 64, 0)
+    assert seg > 0
+
+    def bwd(match, n=seg, dhT=P, dh0=P):
+        _refused("crnn_gated_scan_bwd", 1, P, 64, 64, P, 64, 64, P, 64, 64, None, dhT, P, P, 64, 64, P, 64, 64, dh0, P, n, 1, 16384, 64, 0, None,
+                 match=match)
+    bwd("dh0 == dhT")
+    bwd("workspace", n=seg - 1)

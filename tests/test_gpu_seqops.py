@@ -1132,3 +1132,24 @@ def test_negated_views():
         got = torch.autograd.grad(y, leaves, dy, retain_graph=True)
         for a, b in zip(got, torch.autograd.grad(y, leaves, dy.clone())):
             assert torch.equal(a, b)
+
+
+def test_gated_scan_c_entry_state_gradient_in_place():
+    """dh0 over dhT where the sequence has no segments"""
+    g = gen(101)
+    b, t, d, s = 5, 40, 66, L.stream_ptr()
+    lib = L.lib()
+    assert lib.crnn_gated_scan_workspace(0, b, t, d, 0) == 0
+    f, v, dy, dhT = randn(g, b, t, d), randn(g, b, t, d), randn(g, b, t, d), randn(g, b, d)
+    y, ckpt = torch.empty_like(f), torch.empty(lib.crnn_gated_scan_ckpt_bytes(0, b, t, d, 0) // 4, device=DEV)
+    L.call("crnn_gated_scan_fwd", 0, f.data_ptr(), t * d, d, v.data_ptr(), t * d, d, None, None, y.data_ptr(), t * d, d, None, ckpt.data_ptr(), None,
+           0, b, t, d, 0, s)
+
+    def bwd(din, dout):
+        df, dv = torch.empty_like(f), torch.empty_like(f)
+        L.call("crnn_gated_scan_bwd", 0, dy.data_ptr(), t * d, d, f.data_ptr(), t * d, d, v.data_ptr(), t * d, d, None, din.data_ptr(),
+               ckpt.data_ptr(), df.data_ptr(), t * d, d, dv.data_ptr(), t * d, d, dout.data_ptr(), None, 0, b, t, d, 0, s)
+        return df, dv, dout
+    same = dhT.clone()
+    for a, c in zip(bwd(dhT, torch.empty_like(dhT)), bwd(same, same)):
+        assert torch.equal(a, c)
