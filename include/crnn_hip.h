@@ -563,8 +563,8 @@ int crnn_layernorm_fwd(int dtype, const void* x, long ldx, const float* w, const
                        float* rstd, long M, int N, float eps, void* stream);
 /* dx = rstd (g - mean(g) - xhat mean(g xhat)) (+ dres), g = dy w; dw[n] (+)= sum_m dy xhat, db[n] (+)= sum_m dy
  * (either NULL: not computed). dres (NULL: none): the gradient that reaches x past the norm (a residual branch), added
- * before the one rounding of dx; dx may be dres. ws: crnn_layernorm_bwd_workspace bytes. The sums over rows run in a
- * fixed order (no atomics). */
+ * before the one rounding of dx; dx may be dres, of the same row stride. ws: crnn_layernorm_bwd_workspace bytes. The
+ * sums over rows run in a fixed order (no atomics). */
 size_t crnn_layernorm_bwd_workspace(int dtype, long M, int N);
 int crnn_layernorm_bwd(int dtype, const void* dy, long lddy, const void* x, long ldx, const float* w, const float* mean,
                        const float* rstd, const void* dres, long ldr, void* dx, long lddx, float* dw, float* db,

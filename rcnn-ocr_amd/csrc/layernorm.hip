@@ -580,6 +580,8 @@ int crnn_layernorm_bwd(int dtype, const void* dy, long lddy, const void* x, long
   if (dtype != CRNN_F32 && dtype != CRNN_BF16) return crnn_set_error(hipErrorInvalidValue, "layernorm_bwd: dtype fp32 or bf16");
   if (M < 0 || N < 1 || N > kMaxN || lddy < N || ldx < N || (dx && lddx < N) || (dres && ldr < N))
     return crnn_set_error(hipErrorInvalidValue, "layernorm_bwd: M >= 0, 1 <= N <= 2^30, ld >= N");
+  if (dx && dx == dres && lddx != ldr)   // a row of dx would be written over another row's dres before that is read
+    return crnn_set_error(hipErrorInvalidValue, "layernorm_bwd: dx over dres needs the same row stride");
   if (M > 0 && (!dy || !x || !mean || !rstd)) return crnn_set_error(hipErrorInvalidValue, "layernorm_bwd: null dy / x / mean / rstd");
   if ((dw || db) && (!ws || ws_bytes < crnn_layernorm_bwd_workspace(dtype, M, N)))
     return crnn_set_error(hipErrorInvalidValue, "layernorm_bwd: workspace too small");

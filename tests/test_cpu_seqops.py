@@ -244,3 +244,7 @@ def test_c_gated_scan_bwd_refuses_a_state_gradient_over_its_input():
                  match=match)
     bwd("dh0 == dhT")
     bwd("workspace", n=seg - 1)
+
+
+def test_c_layernorm_bwd_refuses_dx_over_dres_of_another_pitch():
+    _refused("crnn_layernorm_bwd", 0, P, 8, P, 8, None, P, P, P, 9, P, 8, None, None, 0, None, 0, 4, 8, None, match="same row stride")
