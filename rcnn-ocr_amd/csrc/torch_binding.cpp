@@ -44,7 +44,8 @@ void check_type(const char* op, const char* name, const Tensor& t, at::ScalarTyp
 bool has(const OptTensor& t) { return t.has_value() && t->defined(); }
 // The kernels take addresses, so only plain tensors, run at once, will do. Tracers (torch.compile, make_fx, fake tensors), torch.func's
 // derivatives and subclasses with a __torch_dispatch__ are refused: make_fx over real tensors would record the results' allocation and not
-// the kernel that fills them. (torch.vmap calls the operator for each sample on plain tensors.)
+// the kernel that fills them. (torch.vmap calls the operator for each sample on plain tensors;
+// a batch of upstream gradients, is_grads_batched, is refused.)
 void check_eager(const char* op, std::initializer_list<OptTensor> ts) {
   using c10::DispatchKey;
   using Mode = c10::impl::TorchDispatchModeTLS;
@@ -199,6 +200,7 @@ struct LayerNormFn : public torch::autograd::Function<LayerNormFn> {
     {
       at::AutoDispatchBelowADInplaceOrView below;
       const c10::OptionalDeviceGuard guard(x.device());
+      check_eager("layer_norm", {g[0]});
       check_capture("layer_norm");
       const Rows xr = rows(x), dy = rows(g[0]);
       const Tensor w = contiguous(kept[1]), stats = contiguous(kept[2]);
@@ -280,6 +282,7 @@ struct LinearFn : public torch::autograd::Function<LinearFn> {
     {
       at::AutoDispatchBelowADInplaceOrView below;
       const c10::OptionalDeviceGuard guard(x.device());
+      check_eager("linear", {g[0]});
       check_capture("linear");
       if (need_x || need_w || need_b) {
         const int dt = dtype_code("linear", x), act = (int)ctx->saved_data["act"].toInt();
@@ -368,6 +371,7 @@ struct GatedScanFn : public torch::autograd::Function<GatedScanFn> {
     {
       at::AutoDispatchBelowADInplaceOrView below;
       const c10::OptionalDeviceGuard guard(kept[0].device());
+      check_eager("gated_scan", {g[0], g.size() > 1 ? g[1] : Tensor()});
       check_capture("gated_scan");
       const Tensor f = chan(kept[0]), v = chan(kept[1]), len = contiguous(kept[2]), ckpt = contiguous(kept[3]);
       const int dt = dtype_code("gated_scan", f);

@@ -1153,3 +1153,58 @@ def test_gated_scan_c_entry_state_gradient_in_place():
     same = dhT.clone()
     for a, c in zip(bwd(dhT, torch.empty_like(dhT)), bwd(same, same)):
         assert torch.equal(a, c)
+
+
+@pytest.mark.parametrize("op", ["layer_norm", "linear", "gated_scan"])
+def test_batched_upstream_gradients_are_refused(op):
+    fn, x = seq_calls(gen(102))[op]
+    x.requires_grad_(True)
+    y = fn(x)
+    with pytest.raises(RuntimeError, match=f"{op} runs eagerly"):
+        torch.autograd.grad(y, x, torch.ones(3, *y.shape, device=DEV), is_grads_batched=True)
+
+
+@pytest.mark.parametrize("reentrant", [False, True])
+def test_checkpointed_layer(reentrant):
+    """a layer under activation checkpointing (its saved tensors recomputed in the backward): the same gradients"""
+    from torch.utils.checkpoint import checkpoint
+    g = gen(103)
+    x, p = randn(g, 3, 40, 64, dtype=torch.bfloat16), layer_params(g, 64, torch.bfloat16)
+    names = sorted(p)
+    dy = randn(g, 3, 40, 64, dtype=torch.bfloat16)
+
+    def grads(run):
+        leaves = [x.clone().requires_grad_(True)] + [p[k].clone().requires_grad_(True) for k in names]
+        run(lambda x, *w: layer(x, dict(zip(names, w))), leaves).backward(dy)
+        return [t.grad for t in leaves]
+    for a, b in zip(grads(lambda f, t: checkpoint(f, *t, use_reentrant=reentrant)), grads(lambda f, t: f(*t))):
+        assert torch.equal(a, b)
+
+
+def test_graphed_callables():
+    """torch.cuda.make_graphed_callables: forward and backward captured, called in the eager loop with new inputs"""
+    g = gen(104)
+    p = layer_params(g, 64, torch.bfloat16)
+    names = sorted(p)
+
+    class Layer(torch.nn.Module):
+        def __init__(self):
+            super().__init__()
+            self.p = torch.nn.ParameterDict({k: torch.nn.Parameter(p[k].clone()) for k in names})
+
+        def forward(self, x):
+            return layer(x, self.p)
+    plain, captured = Layer(), Layer()
+    sample = randn(g, 3, 40, 64, dtype=torch.bfloat16).requires_grad_(True)
+    graphed = torch.cuda.make_graphed_callables(captured, (sample,))
+    for _ in range(3):
+        x, dy = randn(g, 3, 40, 64, dtype=torch.bfloat16), randn(g, 3, 40, 64, dtype=torch.bfloat16)
+        for m, f in ((plain, plain), (captured, graphed)):
+            m.zero_grad()
+            lx = x.clone().requires_grad_(True)
+            f(lx).backward(dy)
+            m.gx = lx.grad
+        torch.cuda.synchronize()
+        assert torch.equal(plain.gx, captured.gx)
+        for k in names:
+            assert torch.equal(plain.p[k].grad, captured.p[k].grad), k
