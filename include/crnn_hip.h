@@ -585,8 +585,8 @@ size_t crnn_linear_fwd_workspace(int dtype, const void* x, long ldx, const void*
 int crnn_linear_fwd(int dtype, const void* x, long ldx, const void* w, long ldw, const void* bias, int bias_f32, int act,
                     const void* res, long ldr, void* y, long ldy, void* z, long ldz, void* ws, size_t ws_bytes, long M,
                     int N, int K, void* stream);
-/* dz = dy act'(z) (z NULL: act none), dx = dz w, dw (+)= dz^T x, db (+)= sum_m dz; dx, dw, db may each be NULL. dx in
- * dtype; dw fp32 (dw_f32 = 1) or dtype, contiguous [N][K]; db fp32 (db_f32 = 1) or dtype. accumulate needs fp32 dw, db.
+/* dz = dy act'(z) (z NULL: act none), dx = dz w, dw (+)= dz^T x, db (+)= sum_m dz; dx, dw, db may each be NULL. dz is
+ * rounded to dtype for the two products (db adds the unrounded values). dx in dtype; dw fp32 (dw_f32 = 1) or dtype, contiguous [N][K]; db fp32 (db_f32 = 1) or dtype. accumulate needs fp32 dw, db.
  * The sums over rows run in a fixed order. ws: crnn_linear_bwd_workspace bytes. */
 size_t crnn_linear_bwd_workspace(int dtype, const void* dy, long lddy, const void* x, long ldx, const void* w, long ldw,
                                  int act, int need_dx, int need_dw, int need_db, long M, int N, int K);

@@ -25,8 +25,8 @@ def gated_scan(f: torch.Tensor, v: torch.Tensor, h0: Optional[torch.Tensor] = No
     sequence continues. Differentiable once in f, v and h0. Runs on f's device and its current torch stream; capturable
     where lengths is an int32 tensor on the device (another one is converted); a captured backward is refused while an eager
     graph of its leaves, built on the default stream, is alive. ValueError for arguments that do not fit,
-    RuntimeError for CPU
-    tensors and where it is traced (torch.compile, make_fx: torch.compiler.disable keeps it out) or differentiated by torch.func."""
+    RuntimeError for CPU tensors and where it is traced (torch.compile, make_fx: torch.compiler.disable keeps it out) or
+    differentiated by torch.func."""
     global _op
     if _op is None:
         _op = L.ops().gated_scan.default

@@ -434,8 +434,11 @@ int fwd_t(const void* x, long ldx, const void* w, long ldw, const void* bias, in
 
 // ---------------------------------------------------------------- backward
 // dz = dy act'(z) into dz [M][N8] (zero behind N; NULL: only the sums), and the partial column sums part[g][N] of row slice
-// g (NULL: none). A thread owns 8 columns; the 8 row lanes of a workgroup join in LDS. fp32 throughout, dz rounded once to
-// the operands' type for the products; the column sums add the unrounded values.
+// g (NULL: none). A thread owns 8 columns; the 8 row lanes of a workgroup join in LDS. fp32 throughout, the column sums add the unrounded
+// values. dz is rounded once to the operands' type, since the bf16 matrix instructions take nothing else, and z was when it was stored
+// (which halves what this pass reads). Against 64 bits, 8192 x 512 -> 1024 gelu bf16, relative norms: dx and dw 2.4e-3, of which
+// the results' own rounding is 1.66e-3, dz's 1.66e-3 and z's 0.55e-3 (db 1.77e-3). Without them: dz in two bf16 parts, twice the matrix
+// work of dx and dw.
 template <typename T>
 __global__ __launch_bounds__(256) void dz_kernel(const T* __restrict__ dy, long lddy, const T* __restrict__ z, long ldz, int kind,
                                                  T* __restrict__ dz, int N8, float* __restrict__ part, long M, int N) {

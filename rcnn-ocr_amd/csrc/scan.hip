@@ -70,7 +70,7 @@ template <typename T, int VEC, bool FULL> __device__ __forceinline__ void stv(T*
 }
 
 // a = sigmoid(f), r = sigmoid(-f) without cancellation: e = exp(-|f|), the larger is 1 / (1 + e), the smaller e times it.
-// bf16: hardware exp and reciprocal (about 1e-7 relative, far under the inputs' 2^-9); fp32: the exact-rounding forms.
+// bf16: hardware exp and reciprocal (about 1e-7 relative, far under the inputs' 2^-9); fp32: expf (1 ulp) and the IEEE division.
 template <typename T> __device__ __forceinline__ void gate(float f, float& a, float& r) {
   float p, q;
   if constexpr (sizeof(T) == 2) {
@@ -581,7 +581,9 @@ template <typename T, bool BACK> int scan_run(ScanArgs& a, hipStream_t st) {
   if (p.W == 4) return scan_go<T, 4, BACK>(a, st);
   return scan_go<T, kWmax, BACK>(a, st);
 }
-constexpr int kMaxT = 1 << 30;   // step counters are 32 bits and run past T by less than a tile
+// Step counters are 32 bits. The passes run past T by less than a tile, the summaries by less than the last segment, tps tiles: with
+// two segments or more that is at most half of T and a tile, so 2^30 + 2^29 + 64 steps.
+constexpr int kMaxT = 1 << 30;
 bool bad_shape(int dtype, int B, int T, int D, int dir) {
   return (dtype != CRNN_F32 && dtype != CRNN_BF16) || B < 0 || T < 0 || T > kMaxT || D < 0 || D > kMaxT || dir < 0 || dir > 2 || (dir == 2 && D % 2);
 }
