@@ -56,6 +56,34 @@ template <typename T> __device__ __forceinline__ typename VT<T>::v8 zero8() {
   return z;
 }
 
+// ---- rows of any pitch: vectors at element-aligned addresses (gfx950 takes unaligned vector accesses, at the price of the cache
+// lines they straddle)
+typedef bf16x8 bf16x8_u __attribute__((aligned(2)));
+typedef bf16x4 bf16x4_u __attribute__((aligned(2)));
+typedef f32x4 f32x4_u __attribute__((aligned(4)));
+// elements c .. c+7 of a row of n, zero past its end (at most one lane of a row has a part of its 8: for the others the element-wise branch is
+// skipped whole)
+template <typename T> __device__ __forceinline__ typename VT<T>::v8 ld8_row(const T* row, int c, int n) {
+  typename VT<T>::v8 v = zero8<T>();
+  if (c + 8 <= n) {
+    if constexpr (sizeof(T) == 2) {
+      v = *reinterpret_cast<const bf16x8_u*>(row + c);
+    } else {
+      const f32x4 a = *reinterpret_cast<const f32x4_u*>(row + c), b = *reinterpret_cast<const f32x4_u*>(row + c + 4);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        v[i] = a[i];
+        v[4 + i] = b[i];
+      }
+    }
+  } else if (c < n) {
+#pragma unroll
+    for (int i = 0; i < 7; ++i)
+      if (c + i < n) v[i] = row[c + i];
+  }
+  return v;
+}
+
 // 8 elements -> floats, and back
 template <typename T>
 __device__ __forceinline__ void unpack8(const typename VT<T>::v8& v, float* f) {

@@ -16,36 +16,8 @@
 
 namespace {
 
-// 8 elements at an address aligned to the element only (odd row pitches): one or two unaligned 16-byte accesses
-typedef bf16x8 bf16x8_u __attribute__((aligned(2)));
-typedef f32x4 f32x4_u __attribute__((aligned(4)));
-
-// columns c .. c+7 of a row of n columns, `fill` past its end (at most one lane of a row has a part of its 8 columns: for the
-// others the element-wise branch is skipped whole)
-template <typename T> __device__ __forceinline__ typename VT<T>::v8 ldraw8(const T* row, int c, int n, float fill) {
-  typename VT<T>::v8 v;
-#pragma unroll
-  for (int i = 0; i < 8; ++i) v[i] = fromf<T>(fill);
-  if (c + 8 <= n) {
-    if constexpr (sizeof(T) == 2) {
-      v = *reinterpret_cast<const bf16x8_u*>(row + c);
-    } else {
-      const f32x4 a = *reinterpret_cast<const f32x4_u*>(row + c), b = *reinterpret_cast<const f32x4_u*>(row + c + 4);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        v[i] = a[i];
-        v[4 + i] = b[i];
-      }
-    }
-  } else if (c < n) {
-#pragma unroll
-    for (int i = 0; i < 7; ++i)
-      if (c + i < n) v[i] = row[c + i];
-  }
-  return v;
-}
-template <typename T> __device__ __forceinline__ void ldrow8(const T* row, int c, int n, float* f, float fill) {
-  unpack8<T>(ldraw8<T>(row, c, n, fill), f);
+template <typename T> __device__ __forceinline__ void ldrow8(const T* row, int c, int n, float* f) {
+  unpack8<T>(ld8_row<T>(row, c, n), f);
 }
 template <typename T> __device__ __forceinline__ void strow8(T* row, int c, int n, const float* f) {
   if (c + 8 <= n) {
@@ -146,8 +118,8 @@ __global__ __launch_bounds__(ln_threads<WPR>()) void ln_fwd_kernel(const T* __re
       wv[k][i] = 1.f;
       bv[k][i] = 0.f;
     }
-    if (w) ldrow8<float>(w, c[k], N, wv[k], 0.f);
-    if (b) ldrow8<float>(b, c[k], N, bv[k], 0.f);
+    if (w) ldrow8<float>(w, c[k], N, wv[k]);
+    if (b) ldrow8<float>(b, c[k], N, bv[k]);
   }
   constexpr long RPB = ln_rpb<WPR, LPR>();
   for (long mb = (long)blockIdx.x * RPB + (WPR == 1 ? wid * (64 / LPR) : 0); mb < M; mb += (long)gridDim.x * RPB) {
@@ -155,7 +127,7 @@ __global__ __launch_bounds__(ln_threads<WPR>()) void ln_fwd_kernel(const T* __re
     const int n = LPR == 64 || m < M ? N : 0;   // columns of this lane's row: none past the last one
     float v[KC][8];
 #pragma unroll
-    for (int k = 0; k < KC; ++k) ldrow8<T>(x + m * ldx, c[k], n, v[k], 0.f);
+    for (int k = 0; k < KC; ++k) ldrow8<T>(x + m * ldx, c[k], n, v[k]);
     float mu, rs;
     row_stats<WPR, KC, LPR>(v, c, N, eps, red, wr, mu, rs);
     if (mean && lr == 0 && wr == 0 && (LPR == 64 || n)) {
@@ -195,7 +167,7 @@ __global__ __launch_bounds__(ln_threads<WPR>(), WPR == 1 ? 3 : 1) void ln_bwd_ke
       wv[k][i] = 1.f;
       sw[k][i] = sb[k][i] = 0.f;
     }
-    if (w) ldrow8<float>(w, c[k], N, wv[k], 0.f);
+    if (w) ldrow8<float>(w, c[k], N, wv[k]);
   }
   int set = 0;
   constexpr long RPB = ln_rpb<WPR, LPR>();
@@ -206,8 +178,8 @@ __global__ __launch_bounds__(ln_threads<WPR>(), WPR == 1 ? 3 : 1) void ln_bwd_ke
     const int n = LPR == 64 || m < M ? N : 0;
 #pragma unroll
     for (int k = 0; k < KC; ++k) {
-      xr[k] = ldraw8<T>(x + m * ldx, c[k], n, 0.f);
-      gr[k] = ldraw8<T>(dy + m * lddy, c[k], n, 0.f);
+      xr[k] = ld8_row<T>(x + m * ldx, c[k], n);
+      gr[k] = ld8_row<T>(dy + m * lddy, c[k], n);
     }
   };
   if (mb < M) fetch(mb + sub);
@@ -246,7 +218,7 @@ __global__ __launch_bounds__(ln_threads<WPR>(), WPR == 1 ? 3 : 1) void ln_bwd_ke
         for (int i = 0; i < 8; ++i) g[k][i] = rs * (g[k][i] - s1 - xh[k][i] * s2);
         if (dres) {
           float r[8];
-          ldrow8<T>(dres + m * ldr, c[k], n, r, 0.f);
+          ldrow8<T>(dres + m * ldr, c[k], n, r);
 #pragma unroll
           for (int i = 0; i < 8; ++i) g[k][i] += r[i];
         }

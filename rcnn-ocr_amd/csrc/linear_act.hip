@@ -14,32 +14,7 @@ using namespace gemm;
 
 namespace {
 
-// ---------------------------------------------------------------- vectors at element-aligned addresses
-// (rows of any pitch: gfx950 takes unaligned vector accesses, at the price of the cache lines they straddle)
-typedef bf16x8 bf16x8_u __attribute__((aligned(2)));
-typedef bf16x4 bf16x4_u __attribute__((aligned(2)));
-typedef f32x4 f32x4_u __attribute__((aligned(4)));
-// elements k .. k+7 of a row of K, zero past its end
-template <typename T> __device__ __forceinline__ typename VT<T>::v8 ldfrag(const T* row, int k, int K) {
-  typename VT<T>::v8 v = zero8<T>();
-  if (k + 8 <= K) {
-    if constexpr (sizeof(T) == 2) {
-      v = *reinterpret_cast<const bf16x8_u*>(row + k);
-    } else {
-      const f32x4 a = *reinterpret_cast<const f32x4_u*>(row + k), b = *reinterpret_cast<const f32x4_u*>(row + k + 4);
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        v[e] = a[e];
-        v[4 + e] = b[e];
-      }
-    }
-  } else if (k < K) {
-#pragma unroll
-    for (int e = 0; e < 7; ++e)
-      if (k + e < K) v[e] = row[k + e];
-  }
-  return v;
-}
+// ---------------------------------------------------------------- four elements at an element-aligned address
 template <typename T> __device__ __forceinline__ f32x4 ld4u(const T* p) {
   if constexpr (sizeof(T) == 4) {
     return *reinterpret_cast<const f32x4_u*>(p);
@@ -245,7 +220,7 @@ template <typename T> __global__ __launch_bounds__(256) void pad_copy_kernel(Pad
   for (long i = blockIdx.x * 256L + threadIdx.x; i < n8; i += gridDim.x * 256L) {
     const long r = i / c8;
     const int c = (int)(i - r * c8) * 8;
-    st8<T>((T*)j.dst + (r * c8 + c / 8) * 8, ldfrag<T>((const T*)j.src + r * j.ld, c, j.cols));
+    st8<T>((T*)j.dst + (r * c8 + c / 8) * 8, ld8_row<T>((const T*)j.src + r * j.ld, c, j.cols));
   }
 }
 // copies the given jobs (src NULL: none)
@@ -271,7 +246,7 @@ template <typename T> struct RowsAny {
   __device__ __forceinline__ Ctx row_ctx(int r) const { return Ctx{r < rows ? p + r * ld : nullptr}; }
   __device__ __forceinline__ Prep prep(int k0) const { return k0; }
   __device__ __forceinline__ typename VT<T>::v8 load(const Ctx& c, Prep k0, int kofs) const {
-    return c.row ? ldfrag<T>(c.row, k0 + kofs, K) : zero8<T>();
+    return c.row ? ld8_row<T>(c.row, k0 + kofs, K) : zero8<T>();
   }
 };
 // .. and at p[k * ld + row], 8 rows per vector
@@ -286,7 +261,7 @@ template <typename T> struct ColsAny {
   __device__ __forceinline__ Prep prep(int k0) const { return k0; }
   __device__ __forceinline__ typename VT<T>::v8 load(const Ctx& c, Prep k0, int kofs) const {
     const int k = k0 + kofs;
-    return k < K ? ldfrag<T>(p + k * ld, c.r8, rows) : zero8<T>();
+    return k < K ? ld8_row<T>(p + k * ld, c.r8, rows) : zero8<T>();
   }
 };
 
@@ -351,9 +326,9 @@ __global__ __launch_bounds__(64 * SKW) void skinny_kernel(const T* __restrict__ 
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       const int k = k0 + u * SKW * 32 + g8;
-      b[u] = ldfrag<T>(wr, k, K);
+      b[u] = ld8_row<T>(wr, k, K);
 #pragma unroll
-      for (int i = 0; i < MT; ++i) a[u][i] = ldfrag<T>(xr[i], k, K);
+      for (int i = 0; i < MT; ++i) a[u][i] = ld8_row<T>(xr[i], k, K);
     }
 #pragma unroll
     for (int u = 0; u < U; ++u)
@@ -457,8 +432,8 @@ __global__ __launch_bounds__(256) void dz_kernel(const T* __restrict__ dy, long 
         const long m = mb + 8L * r * gridDim.y;
         gr[r] = zero8<T>();
         if (m < M) {
-          gr[r] = ldfrag<T>(dy + m * lddy, n, N);
-          if (z) zr[r] = ldfrag<T>(z + m * ldz, n, N);
+          gr[r] = ld8_row<T>(dy + m * lddy, n, N);
+          if (z) zr[r] = ld8_row<T>(z + m * ldz, n, N);
         }
       }
 #pragma unroll
