@@ -46,14 +46,17 @@ bool has(const OptTensor& t) { return t.has_value() && t->defined(); }
 // derivatives and subclasses with a __torch_dispatch__ are refused: make_fx over real tensors would record the results' allocation and not
 // the kernel that fills them. (torch.vmap calls the operator for each sample on plain tensors;
 // a batch of upstream gradients, is_grads_batched, is refused.)
-void check_eager(const char* op, std::initializer_list<OptTensor> ts) {
+bool is_plain(const Tensor& t) {
   using c10::DispatchKey;
-  using Mode = c10::impl::TorchDispatchModeTLS;
-  using Key = c10::impl::TorchDispatchModeKey;
   static constexpr c10::DispatchKeySet wrapped(
       {DispatchKey::Python, DispatchKey::FuncTorchGradWrapper, DispatchKey::FuncTorchBatched, DispatchKey::Functionalize, DispatchKey::Batched});
+  return !t.unsafeGetTensorImpl()->key_set().has_any(wrapped);
+}
+void check_eager(const char* op, std::initializer_list<OptTensor> ts) {
+  using Mode = c10::impl::TorchDispatchModeTLS;
+  using Key = c10::impl::TorchDispatchModeKey;
   bool plain = true;
-  for (const OptTensor& t : ts) plain = plain && !(has(t) && t->unsafeGetTensorImpl()->key_set().has_any(wrapped));
+  for (const OptTensor& t : ts) plain = plain && (!has(t) || is_plain(*t));
   if (Mode::any_modes_set())
     plain = plain && !Mode::get_mode(Key::FAKE) && !Mode::get_mode(Key::PROXY) && !Mode::get_mode(Key::FUNCTIONAL);
   TORCH_CHECK(plain, op, " runs eagerly, on plain tensors: no tracing (torch.compile, make_fx, fake tensors), no torch.func derivatives, no "
@@ -129,9 +132,10 @@ variable_list saved(const char* op, AutogradContext* ctx) {
     const int64_t dev = p[1];
     const at::IntArrayRef shape(p + 2, dim);
     p += 2 + dim;
-    TORCH_CHECK(t.is_cuda() && t.get_device() == dev && t.scalar_type() == type && t.sizes() == shape && t.layout() == at::kStrided, op,
-                ": a saved-tensor hook gave back a ", t.scalar_type(), " tensor of shape ", t.sizes(), " on ", t.device(), " for a ", type,
-                " one of shape ", shape, " on device ", dev);
+    const bool plain = is_plain(t) && t.layout() == at::kStrided;
+    TORCH_CHECK(plain && t.is_cuda() && t.get_device() == dev && t.scalar_type() == type && t.sizes() == shape, op,
+                ": a saved-tensor hook gave back a ", plain ? "" : "wrapped or sparse ", t.scalar_type(), " tensor of shape ", t.sizes(), " on ",
+                t.device(), " for a ", type, " one of shape ", shape, " on device ", dev);
   }
   return ts;
 }

@@ -1208,3 +1208,24 @@ def test_graphed_callables():
         assert torch.equal(plain.gx, captured.gx)
         for k in names:
             assert torch.equal(plain.p[k].grad, captured.p[k].grad), k
+
+
+@pytest.mark.parametrize("op", ["layer_norm", "linear", "gated_scan"])
+def test_saved_tensors_that_are_wrapped_are_refused(op):
+    """a hook that gives back a subclass of its own (no memory of the values behind it), or a sparse tensor"""
+    class Wrapped(torch.Tensor):
+        @staticmethod
+        def __new__(cls, t):
+            return torch.Tensor._make_wrapper_subclass(cls, t.size(), strides=t.stride(), dtype=t.dtype, device=t.device)
+
+        @classmethod
+        def __torch_dispatch__(cls, func, types, args=(), kwargs=None):
+            assert func is torch.ops.aten.detach.default   # torch's own, on what a hook returns
+            return cls(args[0])
+    for change in (Wrapped, lambda t: t.to_sparse()):
+        fn, x = seq_calls(gen(105))[op]
+        x.requires_grad_(True)
+        with torch.autograd.graph.saved_tensors_hooks(lambda t: t, change):
+            y = fn(x)
+        with pytest.raises(RuntimeError, match=f"{op}: a saved-tensor hook gave back a wrapped"):
+            torch.autograd.grad(y, x, torch.ones_like(y))
